@@ -3,8 +3,8 @@
  * LinOSS 2x2 scan kernels.
  *
  * Conventions shared by every entry point:
- *   - all tensors are fp32 device pointers owned by the caller; the library never
- *     allocates device memory.  Workspaces (forward checkpoints, chunk carries)
+ *   - tensors are device pointers owned by the caller, fp32 unless an entry point
+ *     takes their type; the library never allocates device memory.  Workspaces (forward checkpoints, chunk carries)
  *     are caller-owned too; their size comes from the matching *_floats query.
  *   - strides are in elements; the innermost dimension is always unit-stride.
  *   - every call is asynchronous on `stream` (a cudaStream_t) and returns an
@@ -89,7 +89,7 @@ int mmb_selftest_device_wait(int32_t polls, mmb_stream_t stream);
  * checkpoints are fp32 in every case; state and arithmetic are always fp32.
  * bf16 calls need 16-byte aligned activation pointers and dim and every stride
  * a multiple of 8 (MMB_ERR_ALIGN otherwise). */
-enum mmb_dtype { MMB_F32 = 0, MMB_BF16 = 1 };
+enum mmb_dtype { MMB_F32 = 0, MMB_BF16 = 1, MMB_F16 = 2 /* 8-bit entry points only */ };
 
 typedef struct mmb_mmscan_desc {
     int64_t batch, seqlen, dim, dstate;
@@ -480,6 +480,54 @@ int mmb_linoss_sel_bwd(int32_t disc, int64_t batch, int64_t L, int64_t P, const 
                        const int64_t* C_stride, const float* dy, float* dB_re, float* dB_im,
                        float* dC_re, float* dC_im, float* dA_diag, float* ds, float* work,
                        mmb_stream_t stream);
+
+/* =========================================================================
+ * 8-bit rows and checkpoints (no reference counterpart: the reference keeps and
+ * multiplies everything in fp32).  Types are mmb_dtype; row strides (ld*) are
+ * in elements and at least `cols`, except that a missing tensor's is ignored.
+ * rows == 0 is a call without work.  cols <= 16384 (MMB_ERR_UNSUPPORTED).
+ * Rows whose bases and strides are multiples of 16 bytes (8 bytes for int8),
+ * with cols a multiple of 8, take vector loads; any others work too.
+ *
+ * A row or group that holds a NaN or an infinity gets a NaN scale.
+ * ========================================================================= */
+
+/* 8-bit rows: h = x + residual, v = h * weight,
+ *   q = rint(v * 127 / max|v|),   scale[row] = max|v| * rstd / 127,
+ *   rstd = 1 / sqrt(mean(h^2) + eps)   (norm == 0: rstd = 1, plain rows).
+ * residual, weight and h are nullable; res_type is the type of residual and h:
+ * x_type or fp32.  Rows with max|v| < 2^-100 count as zero. */
+int mmb_norm_q8(int64_t rows, int64_t cols, int32_t x_type, const void* x, int64_t ldx,
+                int32_t res_type, const void* residual, int64_t ldr, const float* weight,
+                float eps, int32_t norm, void* h, int64_t ldh, int8_t* q, int64_t ldq,
+                float* scale, mmb_stream_t stream);
+
+/* The norm in training: n = h * rstd * weight in n_type (nullable), and an
+ * 8-bit checkpoint of h in groups of 128 columns (q nullable: none kept):
+ *   q = rint(h / s),   s = scale[row * ceil(cols / 128) + group], the smallest
+ *   power of two >= 2^-100 with max|h| <= 127 s; the kept value is q * s
+ *   (|q| <= 63 where s = 2^122, so that it stays finite).
+ * rstd[row] (nullable) as above.  norm == 0 with n NULL keeps x as it is. */
+int mmb_norm_ck8_fwd(int64_t rows, int64_t cols, int32_t x_type, const void* x, int64_t ldx,
+                     int32_t res_type, const void* residual, int64_t ldr, const float* weight,
+                     float eps, int32_t norm, void* h, int64_t ldh, int32_t n_type, void* n,
+                     int64_t ldn, int8_t* q, int64_t ldq, float* scale, float* rstd,
+                     mmb_stream_t stream);
+
+/* Its backward, from the checkpoint: z = q * s * rstd, g = dn * weight,
+ *   dx = rstd * (g - z * mean(g z)) + dh,   dweight = sum over rows of dn * z.
+ * dh (nullable) and dx are of dx_type: dn_type or fp32.  dweight is nullable;
+ * when wanted, work holds mmb_norm_ck8_bwd_work_floats(rows, cols) floats.
+ * The sums are added in a fixed order: results repeat bit for bit. */
+size_t mmb_norm_ck8_bwd_work_floats(int64_t rows, int64_t cols);
+int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, const void* dn, int64_t lddn,
+                     int32_t dx_type, const void* dh, int64_t lddh, const float* weight,
+                     const int8_t* q, int64_t ldq, const float* scale, const float* rstd, void* dx,
+                     int64_t lddx, float* dweight, float* work, mmb_stream_t stream);
+
+/* out = q * scale: one scale per row (grouped == 0) or per group of 128 columns. */
+int mmb_restore_q8(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq, const float* scale,
+                   int32_t grouped, int32_t out_type, void* out, int64_t ldo, mmb_stream_t stream);
 
 #ifdef __cplusplus
 }

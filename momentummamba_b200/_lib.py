@@ -35,7 +35,7 @@ class MMScanDesc(ctypes.Structure):
     ]
 
 
-MMB_F32, MMB_BF16 = 0, 1
+MMB_F32, MMB_BF16, MMB_F16 = 0, 1, 2
 
 
 class MMScanTensors(ctypes.Structure):
@@ -104,6 +104,17 @@ _SIGNATURES = {
     "mmb_split_tf32": (ctypes.c_int, [_c_p, _c_p, _c_p, _c_i64, _c_p]),
     "mmb_col_dot_f32": (ctypes.c_int, [_c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_i32,
                                        _c_p]),
+    "mmb_norm_q8": (ctypes.c_int, [_c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i64, _c_p,
+                                   _c_f, _c_i32, _c_p, _c_i64, _c_p, _c_i64, _c_p, _c_p]),
+    "mmb_norm_ck8_fwd": (ctypes.c_int, [_c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i64,
+                                        _c_p, _c_f, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i64,
+                                        _c_p, _c_i64, _c_p, _c_p, _c_p]),
+    "mmb_norm_ck8_bwd_work_floats": (_c_size, [_c_i64, _c_i64]),
+    "mmb_norm_ck8_bwd": (ctypes.c_int, [_c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_i32, _c_p, _c_i64,
+                                        _c_p, _c_p, _c_i64, _c_p, _c_p, _c_p, _c_i64, _c_p, _c_p,
+                                        _c_p]),
+    "mmb_restore_q8": (ctypes.c_int, [_c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_i32, _c_i32, _c_p,
+                                      _c_i64, _c_p]),
     "mmb_linoss_work_floats": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "mmb_linoss_fwd": (ctypes.c_int, [_c_i32, _c_i64, _c_i64, _c_i64] + [_c_p] * 6),
     "mmb_linoss_bwd": (ctypes.c_int, [_c_i32, _c_i64, _c_i64, _c_i64] + [_c_p] * 9),
