@@ -529,6 +529,16 @@ int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, const void* dn
 int mmb_restore_q8(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq, const float* scale,
                    int32_t grouped, int32_t out_type, void* out, int64_t ldo, mmb_stream_t stream);
 
+/* Product of 8-bit rows on the tensor cores (tcgen05 kind::i8):
+ *   out[m, n] = (sum_k x[m, k] w[n, k]) * xs[m] * ws[n] (+ bias[n])
+ * x (M, K) tokens with a scale each, w (N, K) a weight with a scale per output
+ * channel; exact integer sums (K <= 131071), fp32 scaling, one rounding to
+ * out_type.  x and w 16-byte aligned, ldx and ldw multiples of 16; out has any
+ * alignment.  bias nullable. */
+int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* xs,
+                const int8_t* w, int64_t ldw, const float* ws, const float* bias, int32_t out_type,
+                void* out, int64_t ldo, mmb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

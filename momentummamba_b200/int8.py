@@ -206,6 +206,53 @@ def quantize_rows(x: torch.Tensor) -> Q8Rows:
     return _norm_q8(x, None, None, 0.0, 0, "quantize_rows")[0]
 
 
+def _tma_rows(t: torch.Tensor) -> torch.Tensor:
+    """int8 (rows, cols) whose rows start on 16-byte boundaries: t itself where they do."""
+    if (t.stride(1) == 1 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and (
+            t.shape[0] == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])):
+        return t
+    out = _empty_q(t.shape[0], t.shape[1], t.device)
+    out.copy_(t)
+    return out
+
+
+def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
+              out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    """x @ w^T (+ bias) of 8-bit rows: x (..., K), w (N, K) -> (..., N) in out_dtype.
+
+    Sums are exact integers (K <= 131071), scaled in fp32 and rounded once.
+    Rows that do not start on 16-byte boundaries (quantize_rows and rms_norm_q8
+    make ones that do) are copied first.  No gradient."""
+    xq, wq = x.q, w.q
+    _lib.require_cuda(xq, x.scale, wq, w.scale, bias)
+    code = _out_type(out_dtype)
+    if wq.dim() != 2 or xq.dim() < 1 or xq.shape[-1] != wq.shape[1]:
+        raise ValueError(f"linear_q8: x (..., K) and w (N, K) must share K, got {tuple(xq.shape)} "
+                         f"and {tuple(wq.shape)}")
+    N, K = wq.shape
+    if not 1 <= K <= 131071 or N < 1:
+        raise ValueError(f"linear_q8: K must be 1..131071 and N at least 1, got K {K}, N {N}")
+    if bias is not None:
+        if bias.shape != (N,):
+            raise ValueError(f"linear_q8: bias must be ({N},), got {tuple(bias.shape)}")
+        bias = bias.detach().float().contiguous()
+    out = torch.empty((*xq.shape[:-1], N), dtype=out_dtype, device=xq.device)
+    if xq.dim() != 2:
+        xq = xq.reshape(-1, K)
+    M = xq.shape[0]
+    if M:
+        xq, wq = _tma_rows(xq), _tma_rows(wq)
+        xs, ws = x.scale.contiguous(), w.scale.contiguous()
+        _call("mmb_gemm_q8", out, M, N, K, xq.data_ptr(), _ld16(xq), xs.data_ptr(), wq.data_ptr(),
+              _ld16(wq), ws.data_ptr(), _p(bias), code, out.data_ptr(), N)
+    return out
+
+
+def _ld16(t: torch.Tensor) -> int:
+    """Row stride for the tensor maps: one row has whichever multiple of 16 holds it."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+
+
 def _norm_ckpt(x, weight, residual, eps, norm, n_dtype, keep, what):
     """(n, h, q, scale, rstd) of one mmb_norm_ck8_fwd call; x and residual checked here."""
     _lib.require_cuda(x, weight, residual)
