@@ -539,6 +539,22 @@ int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
                 const int8_t* w, int64_t ldw, const float* ws, const float* bias, int32_t out_type,
                 void* out, int64_t ldo, mmb_stream_t stream);
 
+/* A linear's weight gradient from an 8-bit checkpoint of its input (tcgen05,
+ * fp32 accumulation):
+ *   dw[n, k] = col[k] * sum_m dy[m, n] * row[m] * q[m, k] * s[m, k / 128]
+ * dy (M, N) of dy_type; q (M, K), scale (M, ceil(K / 128)) as mmb_norm_ck8_fwd
+ * keeps them; row (M) and col (K) nullable: a norm's rstd and weight.  16-bit dy
+ * is multiplied as it is with the kept values in its type (fp16: kept values
+ * beyond its range become infinities); fp32 dy in three bf16 parts (24 bits).
+ * dw (N, K) of out_type.  M == 0 clears dw.  dy and q 16-byte aligned, lddy a
+ * multiple of 16 bytes, ldq of 16.  work (16-byte aligned) holds
+ * mmb_wgrad_ck8_work_floats floats; results repeat bit for bit. */
+size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int32_t dy_type);
+int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, const void* dy, int64_t lddy,
+                  const int8_t* q, int64_t ldq, const float* scale, const float* row,
+                  const float* col, int32_t out_type, void* dw, int64_t ldw, float* work,
+                  mmb_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -117,6 +117,9 @@ _SIGNATURES = {
                                       _c_i64, _c_p]),
     "mmb_gemm_q8": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, _c_p, _c_i64, _c_p, _c_p, _c_i64, _c_p,
                                    _c_p, _c_i32, _c_p, _c_i64, _c_p]),
+    "mmb_wgrad_ck8_work_floats": (_c_size, [_c_i64, _c_i64, _c_i64, _c_i32]),
+    "mmb_wgrad_ck8": (ctypes.c_int, [_c_i64, _c_i64, _c_i64, _c_i32, _c_p, _c_i64, _c_p, _c_i64,
+                                     _c_p, _c_p, _c_p, _c_i32, _c_p, _c_i64, _c_p, _c_p]),
     "mmb_linoss_work_floats": (_c_size, [_c_i64, _c_i64, _c_i64]),
     "mmb_linoss_fwd": (ctypes.c_int, [_c_i32, _c_i64, _c_i64, _c_i64] + [_c_p] * 6),
     "mmb_linoss_bwd": (ctypes.c_int, [_c_i32, _c_i64, _c_i64, _c_i64] + [_c_p] * 9),

@@ -307,6 +307,7 @@ __global__ void __launch_bounds__(G8_NT, 1)
                     for (int j = 0; j < 32; ++j)
                         if (c + j < ncols) orow[j] = O::from_f(v[j]);
                 }
+                __syncwarp();
                 if (c + 32 < ncols) tmem_wait32(rr[cur ^ 1]);
             }
             tc_fence_before();

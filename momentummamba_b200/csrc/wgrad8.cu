@@ -1,0 +1,522 @@
+// A linear's weight gradient from an 8-bit checkpoint of its input, on the
+// sm_100a tensor cores (tcgen05 kind::f16, fp32 accumulation in TMEM):
+//
+//   dw[n, k] = col[k] * sum_m dy[m, n] * row[m] * q[m, k] * s[m, k / 128]
+//
+// q, s: the checkpoint (groups of 128 columns with power-of-two scales); row
+// and col (nullable) are a norm's 1/rms per token and its weight, for a linear
+// that stands behind one: then q * s is the norm's input and nothing else of
+// the norm's output has to be kept.
+//
+// The kept values are never written out: each CTA loads the bytes, widens them
+// in shared memory and multiplies.
+//   * 16-bit dy goes from TMA to the tensor cores as it is; the kept values are
+//     widened to its type.  q * s is exact there (7 bits and a power of two, in
+//     bf16 for any s, in fp16 within its range); with `row` the product
+//     q * s * row is rounded to that type, half a unit of 2^-8 (bf16) or 2^-11
+//     (fp16), below the half step that q itself is off by.
+//   * fp32 dy (times row, in fp32) is split into three bf16 parts, 24 bits in
+//     all, and multiplied with the exact q * s in three MMAs.
+//
+// Tile: 128 columns of the checkpoint (one group: a token has one scale) as the
+// MMA's rows, BN columns of dy as its columns, both "MN-major" (a token's
+// values are contiguous; tokens are the reduction).  The tokens are cut into
+// slices so that tiles x slices fill the GPU; a slice's tile goes to a
+// workspace and w8_sum_kernel adds the slices in a fixed order.  Persistent,
+// one CTA per SM, roles in separate warps over one ring of token blocks:
+// producer, MMA issuer (two TMEM accumulators), converters, four epilogue
+// warps.  Every wait is bounded.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tc_common.cuh"
+
+namespace mmb {
+
+constexpr int W8_BK = 128;  // checkpoint columns of a tile
+constexpr uint32_t W8_SWZ128 = 2;
+
+// MMA of 16-bit operands, both MN-major, fp32 accumulation: M = 128, N = n
+__host__ __device__ constexpr uint32_t w8_idesc(int n, bool bf16) {
+    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | (1u << 15) |
+           (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+                                         uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// Operand layout of BT tokens: blocks of 64 columns, each BT rows (tokens) of
+// 128 bytes with the 128-byte swizzle: 16-byte chunk c of token t lies at chunk
+// c ^ (t % 8).  Step kk is 16 tokens on.
+template <int BT>
+__device__ __forceinline__ uint64_t w8_desc(uint32_t saddr, int kk) {
+    return smem_desc(saddr + kk * 16 * 128, BT * 128, 1024, W8_SWZ128);
+}
+template <int BT>
+__device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
+    return (uint32_t)(block * (BT * 128) + t * 128 + ((c ^ (t & 7)) << 4));
+}
+
+struct W8BF16 {
+    static constexpr bool BF16 = true, F32 = false;
+    static constexpr int BN = 256, BT = 64, R = 4, CW = 4, BYTES = 2;
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+};
+struct W8F16 {
+    static constexpr bool BF16 = false, F32 = false;
+    static constexpr int BN = 256, BT = 64, R = 4, CW = 4, BYTES = 2;
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+        const __half2 t = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&t);
+    }
+};
+struct W8F32 {
+    static constexpr bool BF16 = true, F32 = true;
+    static constexpr int BN = 128, BT = 32, R = 4, CW = 8, BYTES = 4;
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+        return W8BF16::pack2(a, b);
+    }
+};
+template <class D>
+struct W8Smem {
+    static constexpr int DY = D::BT * D::BN * D::BYTES;      // dy as it lies in memory
+    static constexpr int DY3 = D::F32 ? 3 * D::BT * D::BN * 2 : 0;  // its bf16 parts
+    static constexpr int A = D::BT * W8_BK * 2;               // widened checkpoint
+    static constexpr int Q = D::BT * W8_BK;
+    static constexpr int SLOT = DY + DY3 + A + Q;
+    static constexpr size_t BYTES = (size_t)D::R * SLOT + 1024;
+};
+template <class D>
+__host__ __device__ constexpr int w8_threads() { return 32 * (2 + D::CW + 4); }
+
+struct W8Params {
+    int64_t M, N, K;
+    int64_t blocks;  // token blocks of a slice
+    int64_t slices;
+    const float* scale;  // (M, groups)
+    int64_t groups;
+    const float* row;  // nullable
+    const float* col;  // nullable
+    void* dw;          // one slice: the result itself
+    int64_t ldw;
+    int out_type;
+    float* work;  // more slices: (slices, N, ldp) partial sums
+    int64_t ldp;
+    int* err;
+};
+struct W8Maps {
+    CUtensorMap dy, q;
+};
+
+__device__ __forceinline__ void w8_store(void* dw, int64_t at, int out_type, float v) {
+    if (out_type == MMB_F32) static_cast<float*>(dw)[at] = v;
+    else if (out_type == MMB_BF16) static_cast<__nv_bfloat16*>(dw)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(dw)[at] = __float2half_rn(v);
+}
+
+// 4 bytes -> 4 floats: a byte with its sign bit flipped becomes the low mantissa
+// bits of 2^23, from which 2^23 + 128 is taken away
+__device__ __forceinline__ void w8_widen4(uint32_t w, float (&v)[4]) {
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        v[j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + j)) - 8388736.f;
+}
+
+template <class D>
+__global__ void __launch_bounds__(w8_threads<D>(), 1)
+    w8_kernel(const W8Params p, const __grid_constant__ W8Maps maps) {
+    using Sm = W8Smem<D>;
+    constexpr int R = D::R, BN = D::BN, BT = D::BT;
+    constexpr uint32_t IDESC = w8_idesc(BN, D::BF16);
+    extern __shared__ float4 w8_smem4[];
+    __shared__ uint64_t full[R], conv[R], empty[R], acc_full[2], acc_empty[2], drained;
+    __shared__ uint32_t tmem_base_s;
+    __shared__ int abort_s;
+    volatile int* abort = &abort_s;
+    char* smem = reinterpret_cast<char*>(
+        (reinterpret_cast<uintptr_t>(w8_smem4) + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    const int64_t kt = (p.K + W8_BK - 1) / W8_BK, nt = (p.N + BN - 1) / BN;
+    const int64_t tiles = kt * nt, units = tiles * p.slices;
+    const int64_t nblk = (p.M + BT - 1) / BT;
+    // unit u: slice, then tile with k fastest: CTAs that run together share tokens
+    auto unit_of = [&](int64_t u, int64_t& k0, int64_t& n0, int64_t& b0, int& nb) {
+        const int64_t z = u / tiles, t = u % tiles;
+        k0 = (t % kt) * W8_BK;
+        n0 = (t / kt) * BN;
+        b0 = z * p.blocks;
+        nb = (int)(min64(nblk, b0 + p.blocks) - b0);
+    };
+    auto slot_dy = [&](int s) { return smem + s * Sm::SLOT; };
+    auto slot_b = [&](int s) { return smem + s * Sm::SLOT + (D::F32 ? Sm::DY : 0); };
+    auto slot_a = [&](int s) { return smem + s * Sm::SLOT + Sm::DY + Sm::DY3; };
+    auto slot_q = [&](int s) { return smem + s * Sm::SLOT + Sm::DY + Sm::DY3 + Sm::A; };
+
+    if (tid == 0) {
+        abort_s = 0;
+        for (int s = 0; s < R; ++s) {
+            mbar_init(&full[s], 1);
+            mbar_init(&conv[s], 32 * D::CW);
+            mbar_init(&empty[s], 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            mbar_init(&acc_full[a], 1);
+            mbar_init(&acc_empty[a], 128);
+        }
+        mbar_init(&drained, 1);
+        mbar_fence_init();
+    }
+    if (warp == 1) tmem_alloc(&tmem_base_s, 2 * BN);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base_s;
+
+    if (warp == 0) {
+        // ---- producer ----
+        if (lane == 0) {
+            int64_t j = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                int64_t k0, n0, b0;
+                int nb;
+                unit_of(u, k0, n0, b0, nb);
+                for (int b = 0; b < nb; ++b, ++j) {
+                    const int s = (int)(j % R);
+                    if (j >= R) ok = ws_wait(&empty[s], (uint32_t)(((j / R) - 1) & 1), abort, p.err);
+                    if (!ok) break;
+                    const int m0 = (int)((b0 + b) * BT);
+                    mbar_expect_tx(&full[s], Sm::DY + Sm::Q);
+                    if constexpr (D::F32) {
+                        tma_load_3d(slot_dy(s), &maps.dy, (int)n0, m0, 0, &full[s]);
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < BN / 64; ++g)
+                            tma_load_3d(slot_dy(s) + g * BT * 128, &maps.dy, (int)n0 + 64 * g, m0,
+                                        0, &full[s]);
+                    }
+                    tma_load_3d(slot_q(s), &maps.q, (int)k0, m0, 0, &full[s]);
+                }
+            }
+            // copies still in flight land before the CTA leaves
+            for (int64_t q = j - R > 0 ? j - R : 0; q < j; ++q)
+                mbar_wait_polls(&full[q % R], (uint32_t)((q / R) & 1), 1 << 16);
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer ----
+        if (lane == 0) {
+            int64_t j = 0, lt = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++lt) {
+                int64_t k0, n0, b0;
+                int nb;
+                unit_of(u, k0, n0, b0, nb);
+                const int a = (int)(lt & 1);
+                if (lt >= 2) ok = ws_wait(&acc_empty[a], (uint32_t)(((lt / 2) - 1) & 1), abort, p.err);
+                if (!ok) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + (uint32_t)(a * BN);
+                for (int b = 0; b < nb; ++b, ++j) {
+                    const int s = (int)(j % R);
+                    ok = ws_wait(&conv[s], (uint32_t)((j / R) & 1), abort, p.err);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t sa = smem_u32(slot_a(s)), sb = smem_u32(slot_b(s));
+#pragma unroll
+                    for (int part = 0; part < (D::F32 ? 3 : 1); ++part)
+#pragma unroll
+                        for (int kk = 0; kk < BT / 16; ++kk)
+                            umma_f16(acc, w8_desc<BT>(sa, kk),
+                                     w8_desc<BT>(sb + part * (BT * BN * 2), kk), IDESC,
+                                     (b > 0 || part > 0 || kk > 0) ? 1u : 0u);
+                    umma_commit(&empty[s]);
+                }
+                if (ok) umma_commit(&acc_full[a]);
+            }
+            // every MMA this CTA issued has completed before TMEM is freed
+            umma_commit(&drained);
+            mbar_wait_polls(&drained, 0, 1 << 20);
+        }
+    } else if (warp < 2 + D::CW) {
+        // ---- converters ----
+        constexpr int CT = 32 * D::CW;
+        constexpr int PIECES = BT * W8_BK / 16 / CT;  // 16-byte pieces of q a thread and block
+        const int ct = tid - 64;
+        const int piece = ct & 7;  // the piece's 16 columns; token ct / 8 + i * CT / 8
+        const int blk = piece >> 2, c0 = (piece & 3) * 2;
+        int64_t j = 0;
+        bool ok = true;
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            int64_t k0, n0, b0;
+            int nb;
+            unit_of(u, k0, n0, b0, nb);
+            const int64_t g = k0 / W8_BK;
+            // factors of a block's tokens, loaded one block ahead
+            float f[PIECES];
+            auto factors = [&](int64_t b, float (&o)[PIECES]) {
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int64_t m = b * BT + (ct >> 3) + i * (CT / 8);
+                    o[i] = 0.f;
+                    if (m < p.M) {
+                        o[i] = p.scale[m * p.groups + g];
+                        if (!D::F32 && p.row) o[i] *= p.row[m];
+                    }
+                }
+            };
+            factors(b0, f);
+            for (int b = 0; b < nb; ++b, ++j) {
+                const int s = (int)(j % R);
+                float fn[PIECES];
+                if (b + 1 < nb) factors(b0 + b + 1, fn);
+                float rw[D::F32 ? BT * BN / 8 / CT : 1];
+                if constexpr (D::F32) {
+#pragma unroll
+                    for (int i = 0; i < BT * BN / 8 / CT; ++i) {
+                        const int64_t m = (b0 + b) * BT + (ct >> 4) + i * (CT / 16);
+                        rw[i] = p.row && m < p.M ? p.row[m] : 1.f;
+                    }
+                }
+                ok = ws_wait(&full[s], (uint32_t)((j / R) & 1), abort, p.err);
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) {
+                    const int t = (ct >> 3) + i * (CT / 8);
+                    const uint4 w = *reinterpret_cast<const uint4*>(slot_q(s) + t * W8_BK + piece * 16);
+                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+                    uint32_t o[8];
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        float v[4];
+                        w8_widen4(ws[h], v);
+                        o[2 * h] = D::pack2(v[0] * f[i], v[1] * f[i]);
+                        o[2 * h + 1] = D::pack2(v[2] * f[i], v[3] * f[i]);
+                    }
+                    // the two column blocks write their chunks in opposite order:
+                    // 8 neighbouring lanes then touch all 8 chunks of a row
+                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
+                    const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
+                    char* a = slot_a(s);
+                    *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + blk)) = blk ? hi : lo;
+                    *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + 1 - blk)) = blk ? lo : hi;
+                }
+                if constexpr (D::F32) {
+                    // dy * row = high + middle + low, each bf16: 8 values a step
+                    const int c = ct & 15, swap = (ct >> 2) & 1;
+#pragma unroll
+                    for (int i = 0; i < BT * BN / 8 / CT; ++i) {
+                        const int t = (ct >> 4) + i * (CT / 16);
+                        const float4* src =
+                            reinterpret_cast<const float4*>(slot_dy(s) + t * (BN * 4) + c * 32);
+                        const float4 x0 = src[swap], x1 = src[swap ^ 1];
+                        const float4 a = swap ? x1 : x0, e = swap ? x0 : x1;
+                        float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+#pragma unroll
+                        for (int h = 0; h < 8; ++h) v[h] *= rw[i];
+                        char* dst = slot_b(s) + w8_chunk<BT>(c >> 3, t, c & 7);
+#pragma unroll
+                        for (int part = 0; part < 3; ++part) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                o[h] = D::pack2(v[2 * h], v[2 * h + 1]);
+                                v[2 * h] -= bf16_lo(o[h]);
+                                v[2 * h + 1] -= bf16_hi(o[h]);
+                            }
+                            *reinterpret_cast<uint4*>(dst + part * (BT * BN * 2)) =
+                                make_uint4(o[0], o[1], o[2], o[3]);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&conv[s]);
+#pragma unroll
+                for (int i = 0; i < PIECES; ++i) f[i] = fn[i];
+            }
+        }
+    } else {
+        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (columns k) 32q..32q+31 ----
+        const int q = warp & 3;
+        int64_t lt = 0;
+        bool ok = true;
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++lt) {
+            int64_t k0, n0, b0;
+            int nb;
+            unit_of(u, k0, n0, b0, nb);
+            const int a = (int)(lt & 1);
+            const int64_t k = k0 + q * 32 + lane;
+            const float cs = p.slices == 1 && p.col && k < p.K ? p.col[k] : 1.f;
+            ok = ws_wait(&acc_full[a], (uint32_t)((lt / 2) & 1), abort, p.err);
+            if (!ok) break;
+            tc_fence_after();
+            const int ncols = (int)min64(p.N - n0, BN);
+            const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
+            float* pw = p.work ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k : nullptr;
+#pragma unroll 1
+            for (int c = 0; c < ncols; c += 32) {
+                uint32_t r[32];
+                tmem_ld32_issue(trow + (uint32_t)c, r);
+                tmem_wait32(r);
+                if (k >= p.K) {
+                    // nothing of this lane's column is stored
+                } else if (p.slices > 1) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i < ncols) pw[(int64_t)(c + i) * p.ldp] = __uint_as_float(r[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c + i < ncols)
+                            w8_store(p.dw, (n0 + c + i) * p.ldw + k, p.out_type,
+                                     __uint_as_float(r[i]) * cs);
+                }
+                __syncwarp();
+            }
+            tc_fence_before();
+            mbar_arrive(&acc_empty[a]);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 2 * BN);
+    }
+}
+
+// dw[n, k] = col[k] * sum of the slices' [n, k], in order; 4 columns a thread
+__global__ void __launch_bounds__(256)
+    w8_sum_kernel(int64_t N, int64_t K, const float* __restrict__ work, int64_t ldp,
+                  int64_t slices, const float* __restrict__ col, void* dw, int64_t ldw,
+                  int out_type) {
+    const int64_t quads = ldp / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= N * quads) return;
+    const int64_t n = i / quads, k = (i % quads) * 4;
+    const float* w = work + n * ldp + k;
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int64_t z = 0; z < slices; ++z) {
+        const float4 v = *reinterpret_cast<const float4*>(w + z * N * ldp);
+        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+    }
+    const float v[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (k + j < K) w8_store(dw, n * ldw + k + j, out_type, col ? v[j] * col[k + j] : v[j]);
+}
+
+// ---------------------------------------------------------------------------
+// host side
+// ---------------------------------------------------------------------------
+// Slices of the tokens: the count with the least estimated time, a round of
+// units costing its token blocks plus a tile's way out, and every slice one
+// more write and read of the result.
+struct W8Plan {
+    int64_t slices, blocks;
+};
+template <class D>
+static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
+    const int64_t nblk = (M + D::BT - 1) / D::BT;
+    const int64_t tiles = (K + W8_BK - 1) / W8_BK * ((N + D::BN - 1) / D::BN);
+    const double block_us = D::F32 ? 0.22 : 0.30, tile_us = 2.0;
+    const double slice_us = 2.0 * (double)N * (double)K * 4.0 / 5e6;
+    W8Plan best{1, nblk};
+    double least = 1e30;
+    for (int64_t s = 1; s <= nblk && s <= 148; ++s) {
+        const int64_t per = (nblk + s - 1) / s;
+        if ((nblk + per - 1) / per != s) continue;  // the same as a smaller count
+        const int64_t rounds = (tiles * s + 147) / 148;
+        const double t = (double)rounds * ((double)per * block_us + tile_us) +
+                         (s > 1 ? 2.0 + (double)s * slice_us : 0.0);
+        if (t < least) {
+            least = t;
+            best = {s, per};
+        }
+    }
+    return best;
+}
+static int64_t w8_pitch(int64_t K) { return (K + 3) / 4 * 4; }
+
+template <class D>
+static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, int64_t ldq,
+                     cudaStream_t s) {
+    const W8Plan plan = w8_plan<D>(p.M, p.N, p.K);
+    p.slices = plan.slices;
+    p.blocks = plan.blocks;
+    p.ldp = w8_pitch(p.K);
+    if (p.slices > 1 && !p.work) return MMB_ERR_WORKSPACE;
+    W8Maps maps;
+    const bool okd =
+        D::F32 ? mmb_encode_tile_map(&maps.dy, dy, 4, p.N, p.M, 1, lddy, lddy * p.M, D::BN, D::BT, 0)
+               : mmb_encode_tile_map(&maps.dy, dy, 2, p.N, p.M, 1, lddy, lddy * p.M, 64, D::BT, 128);
+    if (!okd || !mmb_encode_tile_map(&maps.q, q, 1, p.K, p.M, 1, ldq, ldq * p.M, W8_BK, D::BT, 0))
+        return MMB_ERR_ALIGN;
+    static int attr[MMB_MAX_DEVICES] = {};
+    const int st = mmb_smem_attr(w8_kernel<D>, W8Smem<D>::BYTES, attr);
+    if (st != MMB_OK) return st;
+    const int64_t units = (p.K + W8_BK - 1) / W8_BK * ((p.N + D::BN - 1) / D::BN) * p.slices;
+    w8_kernel<D><<<(unsigned)min64(units, 148), w8_threads<D>(), W8Smem<D>::BYTES, s>>>(p, maps);
+    const int rc = mmb_launch_status();
+    if (rc != MMB_OK || p.slices == 1) return rc;
+    const int64_t quads = p.N * (p.ldp / 4);
+    w8_sum_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(p.N, p.K, p.work, p.ldp, p.slices,
+                                                                  p.col, p.dw, p.ldw, p.out_type);
+    return mmb_launch_status();
+}
+
+}  // namespace mmb
+
+using namespace mmb;
+
+extern "C" size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int32_t dy_type) {
+    if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
+    const W8Plan plan = dy_type == MMB_F32 ? w8_plan<W8F32>(M, N, K) : w8_plan<W8BF16>(M, N, K);
+    return plan.slices > 1 ? (size_t)plan.slices * (size_t)N * (size_t)w8_pitch(K) : 0;
+}
+
+extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, const void* dy,
+                             int64_t lddy, const int8_t* q, int64_t ldq, const float* scale,
+                             const float* row, const float* col, int32_t out_type, void* dw,
+                             int64_t ldw, float* work, mmb_stream_t stream) {
+    MMB_NVTX("mmb_wgrad_ck8");
+    if (M < 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX)
+        return MMB_ERR_SHAPE;
+    const auto known = [](int t) { return t == MMB_F32 || t == MMB_BF16 || t == MMB_F16; };
+    if (!known(dy_type) || !known(out_type)) return MMB_ERR_UNSUPPORTED;
+    if (!dw) return MMB_ERR_NULL;
+    if (ldw < K) return MMB_ERR_SHAPE;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (M == 0) {
+        const size_t e = out_type == MMB_F32 ? 4 : 2;
+        if (cudaMemset2DAsync(dw, (size_t)ldw * e, 0, (size_t)K * e, (size_t)N, s) != cudaSuccess)
+            return mmb_launch_status();
+        return MMB_OK;
+    }
+    if (!dy || !q || !scale) return MMB_ERR_NULL;
+    if (lddy < N || ldq < K) return MMB_ERR_SHAPE;
+    // TMA: 16-byte aligned bases and row pitches
+    const int64_t eb = dy_type == MMB_F32 ? 4 : 2;
+    if (((uintptr_t)dy & 15) || ((uintptr_t)q & 15) || (lddy * eb) % 16 || (ldq & 15) ||
+        ((uintptr_t)work & 15))
+        return MMB_ERR_ALIGN;
+    W8Params p{};
+    p.M = M; p.N = N; p.K = K;
+    p.scale = scale; p.groups = (K + W8_BK - 1) / W8_BK; p.row = row; p.col = col;
+    p.dw = dw; p.ldw = ldw; p.out_type = out_type; p.work = work;
+    p.err = mmb_device_error_flag();
+    if (dy_type == MMB_F32) return w8_launch<W8F32>(p, dy, lddy, q, ldq, s);
+    if (dy_type == MMB_BF16) return w8_launch<W8BF16>(p, dy, lddy, q, ldq, s);
+    return w8_launch<W8F16>(p, dy, lddy, q, ldq, s);
+}

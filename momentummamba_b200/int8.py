@@ -356,3 +356,57 @@ def rms_norm_ckpt(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     the residual's type (x itself without a residual)."""
     out = RmsNormCkptFn.apply(x, weight, residual, float(eps), out_dtype or x.dtype)
     return out if residual is not None else (out, x)
+
+
+def _tma_grad(dy: torch.Tensor) -> torch.Tensor:
+    """dy (rows, N) whose rows start on 16-byte boundaries: dy itself where they do."""
+    dy = _rows2(dy)
+    size = dy.element_size()
+    if dy.data_ptr() % 16 == 0 and (dy.shape[0] == 1 or dy.stride(0) * size % 16 == 0):
+        return dy
+    unit = 16 // size
+    out = torch.empty((dy.shape[0], (dy.shape[1] + unit - 1) // unit * unit), dtype=dy.dtype,
+                      device=dy.device)[:, : dy.shape[1]]
+    out.copy_(dy)
+    return out
+
+
+def _factor(t: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if t.numel() != n:
+        raise ValueError(f"weight_grad_ckpt: {what} must hold {n} values, got {tuple(t.shape)}")
+    return t.detach().reshape(-1).float().contiguous()
+
+
+def weight_grad_ckpt(dy: torch.Tensor, kept: Ckpt8, row_scale: Optional[torch.Tensor] = None,
+                     col_scale: Optional[torch.Tensor] = None,
+                     out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The weight gradient (N, K) of a linear whose input was kept in 8 bits:
+
+        dw[n, k] = col_scale[k] * sum_m dy[m, n] * row_scale[m] * kept[m, k]
+
+    dy (..., N) fp32, bf16 or fp16 with kept's rows; row_scale (one a row) and
+    col_scale (K,) are a norm's rstd and weight where the linear stands behind
+    one.  In dy's type unless out_dtype says otherwise; sums are fp32."""
+    _lib.require_cuda(dy, kept.q, kept.scale, row_scale, col_scale)
+    code = _type(dy, "weight_grad_ckpt: dy")
+    M, K = kept.q.shape
+    if dy.dim() < 1 or dy.shape[-1] < 1 or dy.numel() != M * dy.shape[-1]:
+        raise ValueError(f"weight_grad_ckpt: dy (..., N) must have the checkpoint's {M} rows, got "
+                         f"{tuple(dy.shape)}")
+    N = dy.shape[-1]
+    row, col = _factor(row_scale, M, "row_scale"), _factor(col_scale, K, "col_scale")
+    out_dtype = out_dtype or dy.dtype
+    oc = _out_type(out_dtype)
+    dw = torch.empty((N, K), dtype=out_dtype, device=dy.device)
+    dy2, q = _tma_grad(dy.detach()), _tma_rows(kept.q)
+    work = None
+    floats = _lib.load().mmb_wgrad_ck8_work_floats(M, N, K, code)
+    if floats:
+        work = torch.empty((floats,), device=dy.device)
+    unit = 16 // dy.element_size()
+    _call("mmb_wgrad_ck8", dy, M, N, K, code, dy2.data_ptr(),
+          dy2.stride(0) if M > 1 else -(-N // unit) * unit, q.data_ptr(), _ld16(q),
+          kept.scale.data_ptr(), _p(row), _p(col), oc, dw.data_ptr(), K, _p(work))
+    return dw
