@@ -63,9 +63,13 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
     return (uint32_t)(block * (BT * 128) + t * 128 + ((c ^ (t & 7)) << 4));
 }
 
+// BN: dy columns of a tile; BT: tokens of a block; RL, RC: blocks in flight as
+// they lie in memory / widened; CW, EW: converter and epilogue warps; SEG: token
+// blocks that accumulate in TMEM before the sums move to registers.
 struct W8BF16 {
     static constexpr bool BF16 = true, F32 = false;
-    static constexpr int BN = 256, BT = 64, R = 4, CW = 4, BYTES = 2;
+    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 4, EW = 4, BYTES = 2;
+    static constexpr int SEG = 1 << 30;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&t);
@@ -73,30 +77,44 @@ struct W8BF16 {
 };
 struct W8F16 {
     static constexpr bool BF16 = false, F32 = false;
-    static constexpr int BN = 256, BT = 64, R = 4, CW = 4, BYTES = 2;
+    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 4, EW = 4, BYTES = 2;
+    static constexpr int SEG = 1 << 30;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         const __half2 t = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&t);
     }
 };
+// The tensor cores' fp32 accumulation truncates: its error grows with the number
+// of steps.  1024 tokens (64 steps) at a time, added to sums in registers with
+// ordinary rounding, and the small parts in an accumulator of their own, keep
+// the result as near as an fp32 product's.
 struct W8F32 {
     static constexpr bool BF16 = true, F32 = true;
-    static constexpr int BN = 128, BT = 32, R = 4, CW = 8, BYTES = 4;
+    static constexpr int BN = 128, BT = 32, RL = 6, RC = 3, CW = 8, EW = 8, BYTES = 4;
+    static constexpr int SEG = 32;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return W8BF16::pack2(a, b);
     }
 };
 template <class D>
 struct W8Smem {
-    static constexpr int DY = D::BT * D::BN * D::BYTES;      // dy as it lies in memory
-    static constexpr int DY3 = D::F32 ? 3 * D::BT * D::BN * 2 : 0;  // its bf16 parts
-    static constexpr int A = D::BT * W8_BK * 2;               // widened checkpoint
+    static constexpr int DY = D::BT * D::BN * D::BYTES;  // dy as it lies in memory
     static constexpr int Q = D::BT * W8_BK;
-    static constexpr int SLOT = DY + DY3 + A + Q;
-    static constexpr size_t BYTES = (size_t)D::R * SLOT + 1024;
+    static constexpr int FACT = 1024;                    // scale and row factor of BT tokens
+    static constexpr int LOAD = DY + Q + FACT;
+    static constexpr int A = D::BT * W8_BK * 2;          // widened checkpoint
+    static constexpr int DY3 = D::F32 ? 3 * D::BT * D::BN * 2 : 0;  // dy's bf16 parts
+    static constexpr int CONV = A + DY3;
+    static constexpr size_t BYTES = (size_t)D::RL * LOAD + (size_t)D::RC * CONV + 1024;
 };
 template <class D>
-__host__ __device__ constexpr int w8_threads() { return 32 * (2 + D::CW + 4); }
+__host__ __device__ constexpr int w8_threads() { return 32 * (2 + D::CW + D::EW); }
+
+// `bar` counts an arrival of this lane once its cp.async copies so far have landed
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
 
 struct W8Params {
     int64_t M, N, K;
@@ -136,10 +154,13 @@ template <class D>
 __global__ void __launch_bounds__(w8_threads<D>(), 1)
     w8_kernel(const W8Params p, const __grid_constant__ W8Maps maps) {
     using Sm = W8Smem<D>;
-    constexpr int R = D::R, BN = D::BN, BT = D::BT;
+    constexpr int RL = D::RL, RC = D::RC, BN = D::BN, BT = D::BT;
+    constexpr int ACC = D::F32 ? 2 * BN : BN;  // TMEM columns of an accumulator
+    constexpr int CT = 32 * D::CW;
     constexpr uint32_t IDESC = w8_idesc(BN, D::BF16);
     extern __shared__ float4 w8_smem4[];
-    __shared__ uint64_t full[R], conv[R], empty[R], acc_full[2], acc_empty[2], drained;
+    __shared__ uint64_t full[RL], free_l[RL], conv[RC], free_c[RC], acc_full[2], acc_empty[2],
+        drained;
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
     volatile int* abort = &abort_s;
@@ -158,91 +179,115 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         b0 = z * p.blocks;
         nb = (int)(min64(nblk, b0 + p.blocks) - b0);
     };
-    auto slot_dy = [&](int s) { return smem + s * Sm::SLOT; };
-    auto slot_b = [&](int s) { return smem + s * Sm::SLOT + (D::F32 ? Sm::DY : 0); };
-    auto slot_a = [&](int s) { return smem + s * Sm::SLOT + Sm::DY + Sm::DY3; };
-    auto slot_q = [&](int s) { return smem + s * Sm::SLOT + Sm::DY + Sm::DY3 + Sm::A; };
+    auto slot_dy = [&](int s) { return smem + s * Sm::LOAD; };
+    auto slot_q = [&](int s) { return smem + s * Sm::LOAD + Sm::DY; };
+    auto slot_f = [&](int s) {
+        return reinterpret_cast<float*>(smem + s * Sm::LOAD + Sm::DY + Sm::Q);
+    };
+    auto slot_a = [&](int c) { return smem + RL * Sm::LOAD + c * Sm::CONV; };
+    auto slot_dy3 = [&](int c) { return smem + RL * Sm::LOAD + c * Sm::CONV + Sm::A; };
 
     if (tid == 0) {
         abort_s = 0;
-        for (int s = 0; s < R; ++s) {
-            mbar_init(&full[s], 1);
-            mbar_init(&conv[s], 32 * D::CW);
-            mbar_init(&empty[s], 1);
+        for (int s = 0; s < RL; ++s) {
+            mbar_init(&full[s], 1 + 32);               // TMA, and the factors of each lane
+            mbar_init(&free_l[s], D::F32 ? CT : 1);    // read by the converters / by the MMAs
+        }
+        for (int c = 0; c < RC; ++c) {
+            mbar_init(&conv[c], CT);
+            mbar_init(&free_c[c], 1);
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&acc_full[a], 1);
-            mbar_init(&acc_empty[a], 128);
+            mbar_init(&acc_empty[a], 32 * D::EW);
         }
         mbar_init(&drained, 1);
         mbar_fence_init();
     }
-    if (warp == 1) tmem_alloc(&tmem_base_s, 2 * BN);
+    if (warp == 1) tmem_alloc(&tmem_base_s, 2 * ACC);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = tmem_base_s;
 
     if (warp == 0) {
-        // ---- producer ----
+        // ---- producer: tiles by TMA (lane 0), the tokens' factors by cp.async ----
+        int64_t j = 0;
+        bool ok = true;
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+            int64_t k0, n0, b0;
+            int nb;
+            unit_of(u, k0, n0, b0, nb);
+            const int64_t g = k0 / W8_BK;
+            for (int b = 0; b < nb; ++b, ++j) {
+                const int s = (int)(j % RL);
+                if (j >= RL) ok = ws_wait(&free_l[s], (uint32_t)(((j / RL) - 1) & 1), abort, p.err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const int64_t m0 = (b0 + b) * BT;
+                if (lane == 0) {
+                    mbar_expect_tx(&full[s], Sm::DY + Sm::Q);
+                    if constexpr (D::F32) {
+                        tma_load_3d(slot_dy(s), &maps.dy, (int)n0, (int)m0, 0, &full[s]);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c)
+                            tma_load_3d(slot_dy(s) + c * BT * 128, &maps.dy, (int)n0 + 64 * c,
+                                        (int)m0, 0, &full[s]);
+                    }
+                    tma_load_3d(slot_q(s), &maps.q, (int)k0, (int)m0, 0, &full[s]);
+                }
+                for (int t = lane; t < BT; t += 32) {
+                    const int64_t m = m0 + t;
+                    const bool in = m < p.M;
+                    cp_async4(slot_f(s) + t, in ? p.scale + m * p.groups + g : p.scale, in);
+                    if (p.row) cp_async4(slot_f(s) + 128 + t, in ? p.row + m : p.row, in);
+                }
+                cp_async_arrive(&full[s]);
+            }
+        }
+        // copies still in flight land before the CTA leaves
+        for (int64_t q = j - RL > 0 ? j - RL : 0; q < j; ++q)
+            mbar_wait_polls(&full[q % RL], (uint32_t)((q / RL) & 1), 1 << 16);
+    } else if (warp == 1) {
+        // ---- MMA issuer ----
         if (lane == 0) {
-            int64_t j = 0;
+            int64_t j = 0, seg = 0;
             bool ok = true;
             for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 int64_t k0, n0, b0;
                 int nb;
                 unit_of(u, k0, n0, b0, nb);
                 for (int b = 0; b < nb; ++b, ++j) {
-                    const int s = (int)(j % R);
-                    if (j >= R) ok = ws_wait(&empty[s], (uint32_t)(((j / R) - 1) & 1), abort, p.err);
-                    if (!ok) break;
-                    const int m0 = (int)((b0 + b) * BT);
-                    mbar_expect_tx(&full[s], Sm::DY + Sm::Q);
-                    if constexpr (D::F32) {
-                        tma_load_3d(slot_dy(s), &maps.dy, (int)n0, m0, 0, &full[s]);
-                    } else {
-#pragma unroll
-                        for (int g = 0; g < BN / 64; ++g)
-                            tma_load_3d(slot_dy(s) + g * BT * 128, &maps.dy, (int)n0 + 64 * g, m0,
-                                        0, &full[s]);
+                    const int a = (int)(seg & 1);
+                    const int in_seg = b % D::SEG;
+                    if (in_seg == 0) {
+                        if (seg >= 2)
+                            ok = ws_wait(&acc_empty[a], (uint32_t)(((seg / 2) - 1) & 1), abort, p.err);
+                        if (!ok) break;
+                        tc_fence_after();
                     }
-                    tma_load_3d(slot_q(s), &maps.q, (int)k0, m0, 0, &full[s]);
-                }
-            }
-            // copies still in flight land before the CTA leaves
-            for (int64_t q = j - R > 0 ? j - R : 0; q < j; ++q)
-                mbar_wait_polls(&full[q % R], (uint32_t)((q / R) & 1), 1 << 16);
-        }
-    } else if (warp == 1) {
-        // ---- MMA issuer ----
-        if (lane == 0) {
-            int64_t j = 0, lt = 0;
-            bool ok = true;
-            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++lt) {
-                int64_t k0, n0, b0;
-                int nb;
-                unit_of(u, k0, n0, b0, nb);
-                const int a = (int)(lt & 1);
-                if (lt >= 2) ok = ws_wait(&acc_empty[a], (uint32_t)(((lt / 2) - 1) & 1), abort, p.err);
-                if (!ok) break;
-                tc_fence_after();
-                const uint32_t acc = tmem + (uint32_t)(a * BN);
-                for (int b = 0; b < nb; ++b, ++j) {
-                    const int s = (int)(j % R);
-                    ok = ws_wait(&conv[s], (uint32_t)((j / R) & 1), abort, p.err);
+                    const uint32_t acc = tmem + (uint32_t)(a * ACC);
+                    const int s = (int)(j % RL), c = (int)(j % RC);
+                    ok = ws_wait(&conv[c], (uint32_t)((j / RC) & 1), abort, p.err);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(slot_a(s)), sb = smem_u32(slot_b(s));
+                    const uint32_t sa = smem_u32(slot_a(c));
+                    const uint32_t sb = smem_u32(D::F32 ? slot_dy3(c) : slot_dy(s));
 #pragma unroll
                     for (int part = 0; part < (D::F32 ? 3 : 1); ++part)
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk)
-                            umma_f16(acc, w8_desc<BT>(sa, kk),
+                            umma_f16(acc + (part ? BN : 0), w8_desc<BT>(sa, kk),
                                      w8_desc<BT>(sb + part * (BT * BN * 2), kk), IDESC,
-                                     (b > 0 || part > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&empty[s]);
+                                     (in_seg > 0 || part == 2 || kk > 0) ? 1u : 0u);
+                    if constexpr (!D::F32) umma_commit(&free_l[s]);
+                    umma_commit(&free_c[c]);
+                    if (in_seg == D::SEG - 1 || b == nb - 1) {
+                        umma_commit(&acc_full[a]);
+                        ++seg;
+                    }
                 }
-                if (ok) umma_commit(&acc_full[a]);
             }
             // every MMA this CTA issued has completed before TMEM is freed
             umma_commit(&drained);
@@ -250,7 +295,6 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         }
     } else if (warp < 2 + D::CW) {
         // ---- converters ----
-        constexpr int CT = 32 * D::CW;
         constexpr int PIECES = BT * W8_BK / 16 / CT;  // 16-byte pieces of q a thread and block
         const int ct = tid - 64;
         const int piece = ct & 7;  // the piece's 16 columns; token ct / 8 + i * CT / 8
@@ -261,53 +305,31 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            const int64_t g = k0 / W8_BK;
-            // factors of a block's tokens, loaded one block ahead
-            float f[PIECES];
-            auto factors = [&](int64_t b, float (&o)[PIECES]) {
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
-                    const int64_t m = b * BT + (ct >> 3) + i * (CT / 8);
-                    o[i] = 0.f;
-                    if (m < p.M) {
-                        o[i] = p.scale[m * p.groups + g];
-                        if (!D::F32 && p.row) o[i] *= p.row[m];
-                    }
-                }
-            };
-            factors(b0, f);
             for (int b = 0; b < nb; ++b, ++j) {
-                const int s = (int)(j % R);
-                float fn[PIECES];
-                if (b + 1 < nb) factors(b0 + b + 1, fn);
-                float rw[D::F32 ? BT * BN / 8 / CT : 1];
-                if constexpr (D::F32) {
-#pragma unroll
-                    for (int i = 0; i < BT * BN / 8 / CT; ++i) {
-                        const int64_t m = (b0 + b) * BT + (ct >> 4) + i * (CT / 16);
-                        rw[i] = p.row && m < p.M ? p.row[m] : 1.f;
-                    }
-                }
-                ok = ws_wait(&full[s], (uint32_t)((j / R) & 1), abort, p.err);
+                const int s = (int)(j % RL), cs = (int)(j % RC);
+                if (j >= RC) ok = ws_wait(&free_c[cs], (uint32_t)(((j / RC) - 1) & 1), abort, p.err);
+                if (ok) ok = ws_wait(&full[s], (uint32_t)((j / RL) & 1), abort, p.err);
                 if (!ok) break;
+                const float* fs = slot_f(s);
 #pragma unroll
                 for (int i = 0; i < PIECES; ++i) {
                     const int t = (ct >> 3) + i * (CT / 8);
                     const uint4 w = *reinterpret_cast<const uint4*>(slot_q(s) + t * W8_BK + piece * 16);
+                    const float f = !D::F32 && p.row ? fs[t] * fs[128 + t] : fs[t];
                     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
                     uint32_t o[8];
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
                         float v[4];
                         w8_widen4(ws[h], v);
-                        o[2 * h] = D::pack2(v[0] * f[i], v[1] * f[i]);
-                        o[2 * h + 1] = D::pack2(v[2] * f[i], v[3] * f[i]);
+                        o[2 * h] = D::pack2(v[0] * f, v[1] * f);
+                        o[2 * h + 1] = D::pack2(v[2] * f, v[3] * f);
                     }
                     // the two column blocks write their chunks in opposite order:
                     // 8 neighbouring lanes then touch all 8 chunks of a row
                     const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
                     const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
-                    char* a = slot_a(s);
+                    char* a = slot_a(cs);
                     *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + blk)) = blk ? hi : lo;
                     *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + 1 - blk)) = blk ? lo : hi;
                 }
@@ -322,9 +344,12 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                         const float4 x0 = src[swap], x1 = src[swap ^ 1];
                         const float4 a = swap ? x1 : x0, e = swap ? x0 : x1;
                         float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+                        if (p.row) {
+                            const float r = fs[128 + t];
 #pragma unroll
-                        for (int h = 0; h < 8; ++h) v[h] *= rw[i];
-                        char* dst = slot_b(s) + w8_chunk<BT>(c >> 3, t, c & 7);
+                            for (int h = 0; h < 8; ++h) v[h] *= r;
+                        }
+                        char* dst = slot_dy3(cs) + w8_chunk<BT>(c >> 3, t, c & 7);
 #pragma unroll
                         for (int part = 0; part < 3; ++part) {
                             uint32_t o[4];
@@ -340,58 +365,85 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&conv[s]);
-#pragma unroll
-                for (int i = 0; i < PIECES; ++i) f[i] = fn[i];
+                mbar_arrive(&conv[cs]);
+                if constexpr (D::F32) mbar_arrive(&free_l[s]);
             }
         }
     } else {
-        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (columns k) 32q..32q+31 ----
+        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (columns k) 32q..32q+31,
+        // every 4 warps a share of the columns n ----
         const int q = warp & 3;
-        int64_t lt = 0;
+        constexpr int COLS = BN / (D::EW / 4);
+        const int col0 = ((warp - 2 - D::CW) >> 2) * COLS;
+        int64_t seg = 0;
         bool ok = true;
-        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x, ++lt) {
+        for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            const int a = (int)(lt & 1);
             const int64_t k = k0 + q * 32 + lane;
             const float cs = p.slices == 1 && p.col && k < p.K ? p.col[k] : 1.f;
-            ok = ws_wait(&acc_full[a], (uint32_t)((lt / 2) & 1), abort, p.err);
-            if (!ok) break;
-            tc_fence_after();
             const int ncols = (int)min64(p.N - n0, BN);
-            const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
             float* pw = p.work ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k : nullptr;
-#pragma unroll 1
-            for (int c = 0; c < ncols; c += 32) {
-                uint32_t r[32];
-                tmem_ld32_issue(trow + (uint32_t)c, r);
-                tmem_wait32(r);
-                if (k >= p.K) {
-                    // nothing of this lane's column is stored
-                } else if (p.slices > 1) {
+            const auto put = [&](int c, float v) {
+                if (c >= ncols || k >= p.K) return;
+                if (p.slices > 1) pw[(int64_t)c * p.ldp] = v;
+                else w8_store(p.dw, (n0 + c) * p.ldw + k, p.out_type, v * cs);
+            };
+            if constexpr (D::F32) {
+                float sum[COLS];
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c + i < ncols) pw[(int64_t)(c + i) * p.ldp] = __uint_as_float(r[i]);
-                } else {
+                for (int i = 0; i < COLS; ++i) sum[i] = 0.f;
+                for (int b = 0; b < nb; b += D::SEG, ++seg) {
+                    const int a = (int)(seg & 1);
+                    ok = ws_wait(&acc_full[a], (uint32_t)((seg / 2) & 1), abort, p.err);
+                    ok = __all_sync(0xffffffffu, ok);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t trow =
+                        tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC + col0);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c + i < ncols)
-                            w8_store(p.dw, (n0 + c + i) * p.ldw + k, p.out_type,
-                                     __uint_as_float(r[i]) * cs);
+                    for (int h = 0; h < 2; ++h)  // the small parts, then the high ones
+#pragma unroll
+                        for (int c = 0; c < COLS; c += 16) {
+                            float r[16];
+                            tmem_ld16(trow + (uint32_t)((h ? 0 : BN) + c), r);
+#pragma unroll
+                            for (int i = 0; i < 16; ++i) sum[c + i] += r[i];
+                        }
+                    tc_fence_before();
+                    mbar_arrive(&acc_empty[a]);
                 }
-                __syncwarp();
+                if (!ok) break;
+#pragma unroll
+                for (int i = 0; i < COLS; ++i) put(col0 + i, sum[i]);
+            } else {
+                const int a = (int)(seg & 1);
+                ok = ws_wait(&acc_full[a], (uint32_t)((seg / 2) & 1), abort, p.err);
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                ++seg;
+                tc_fence_after();
+                const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC);
+#pragma unroll 1
+                for (int c = 0; c < ncols; c += 32) {
+                    uint32_t r[32];
+                    tmem_ld32_issue(trow + (uint32_t)c, r);
+                    tmem_wait32(r);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) put(c + i, __uint_as_float(r[i]));
+                    __syncwarp();
+                }
+                tc_fence_before();
+                mbar_arrive(&acc_empty[a]);
             }
-            tc_fence_before();
-            mbar_arrive(&acc_empty[a]);
         }
     }
     tc_fence_before();
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * BN);
+        tmem_dealloc(tmem, 2 * ACC);
     }
 }
 
