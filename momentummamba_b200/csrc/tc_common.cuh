@@ -129,4 +129,19 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// A place in a ring of R slots and the phase of its barriers.  The side that
+// fills waits for the opposite phase: a fresh barrier counts as having passed
+// the phase before its first.
+template <int R>
+struct RingPos {
+    int s = 0;
+    uint32_t ph = 0;
+    __device__ __forceinline__ void next() {
+        if (++s == R) {
+            s = 0;
+            ph ^= 1u;
+        }
+    }
+};
+
 }  // namespace mmb

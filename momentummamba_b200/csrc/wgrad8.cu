@@ -68,7 +68,7 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 // blocks that accumulate in TMEM before the sums move to registers.
 struct W8BF16 {
     static constexpr bool BF16 = true, F32 = false;
-    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 4, EW = 4, BYTES = 2;
+    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 8, EW = 4, BYTES = 2;
     static constexpr int SEG = 1 << 30;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
@@ -77,7 +77,7 @@ struct W8BF16 {
 };
 struct W8F16 {
     static constexpr bool BF16 = false, F32 = false;
-    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 4, EW = 4, BYTES = 2;
+    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 8, EW = 4, BYTES = 2;
     static constexpr int SEG = 1 << 30;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         const __half2 t = __floats2half2_rn(a, b);
@@ -143,11 +143,11 @@ __device__ __forceinline__ void w8_store(void* dw, int64_t at, int out_type, flo
 
 // 4 bytes -> 4 floats: a byte with its sign bit flipped becomes the low mantissa
 // bits of 2^23, from which 2^23 + 128 is taken away
-__device__ __forceinline__ void w8_widen4(uint32_t w, float (&v)[4]) {
+__device__ __forceinline__ void w8_widen4(uint32_t w, float2& v0, float2& v1) {
     const uint32_t u = w ^ 0x80808080u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        v[j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + j)) - 8388736.f;
+    const auto at = [&](int j) { return __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + j)); };
+    v0 = fadd2(make_float2(at(0), at(1)), f2(-8388736.f));
+    v1 = fadd2(make_float2(at(2), at(3)), f2(-8388736.f));
 }
 
 template <class D>
@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 
     if (warp == 0) {
         // ---- producer: tiles by TMA (lane 0), the tokens' factors by cp.async ----
+        RingPos<RL> r;
         int64_t j = 0;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -219,10 +220,9 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             int nb;
             unit_of(u, k0, n0, b0, nb);
             const int64_t g = k0 / W8_BK;
-            for (int b = 0; b < nb; ++b, ++j) {
-                const int s = (int)(j % RL);
-                if (j >= RL) ok = ws_wait(&free_l[s], (uint32_t)(((j / RL) - 1) & 1), abort, p.err);
-                ok = __all_sync(0xffffffffu, ok);
+            for (int b = 0; b < nb; ++b, ++j, r.next()) {
+                const int s = r.s;
+                ok = __all_sync(0xffffffffu, ws_wait(&free_l[s], r.ph ^ 1u, abort, p.err));
                 if (!ok) break;
                 const int64_t m0 = (b0 + b) * BT;
                 if (lane == 0) {
@@ -252,24 +252,25 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     } else if (warp == 1) {
         // ---- MMA issuer ----
         if (lane == 0) {
-            int64_t j = 0, seg = 0;
+            RingPos<RL> rl;
+            RingPos<RC> rc;
+            RingPos<2> ra;
             bool ok = true;
             for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 int64_t k0, n0, b0;
                 int nb;
                 unit_of(u, k0, n0, b0, nb);
-                for (int b = 0; b < nb; ++b, ++j) {
-                    const int a = (int)(seg & 1);
+                for (int b = 0; b < nb; ++b, rl.next(), rc.next()) {
+                    const int a = ra.s;
                     const int in_seg = b % D::SEG;
                     if (in_seg == 0) {
-                        if (seg >= 2)
-                            ok = ws_wait(&acc_empty[a], (uint32_t)(((seg / 2) - 1) & 1), abort, p.err);
+                        ok = ws_wait(&acc_empty[a], ra.ph ^ 1u, abort, p.err);
                         if (!ok) break;
                         tc_fence_after();
                     }
                     const uint32_t acc = tmem + (uint32_t)(a * ACC);
-                    const int s = (int)(j % RL), c = (int)(j % RC);
-                    ok = ws_wait(&conv[c], (uint32_t)((j / RC) & 1), abort, p.err);
+                    const int s = rl.s, c = rc.s;
+                    ok = ws_wait(&conv[c], rc.ph, abort, p.err);
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t sa = smem_u32(slot_a(c));
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     umma_commit(&free_c[c]);
                     if (in_seg == D::SEG - 1 || b == nb - 1) {
                         umma_commit(&acc_full[a]);
-                        ++seg;
+                        ra.next();
                     }
                 }
             }
@@ -299,16 +300,17 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         const int ct = tid - 64;
         const int piece = ct & 7;  // the piece's 16 columns; token ct / 8 + i * CT / 8
         const int blk = piece >> 2, c0 = (piece & 3) * 2;
-        int64_t j = 0;
+        RingPos<RL> rl;
+        RingPos<RC> rc;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            for (int b = 0; b < nb; ++b, ++j) {
-                const int s = (int)(j % RL), cs = (int)(j % RC);
-                if (j >= RC) ok = ws_wait(&free_c[cs], (uint32_t)(((j / RC) - 1) & 1), abort, p.err);
-                if (ok) ok = ws_wait(&full[s], (uint32_t)((j / RL) & 1), abort, p.err);
+            for (int b = 0; b < nb; ++b, rl.next(), rc.next()) {
+                const int s = rl.s, cs = rc.s;
+                ok = ws_wait(&free_c[cs], rc.ph ^ 1u, abort, p.err) &&
+                     ws_wait(&full[s], rl.ph, abort, p.err);
                 if (!ok) break;
                 const float* fs = slot_f(s);
 #pragma unroll
@@ -320,10 +322,12 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     uint32_t o[8];
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        float v[4];
-                        w8_widen4(ws[h], v);
-                        o[2 * h] = D::pack2(v[0] * f, v[1] * f);
-                        o[2 * h + 1] = D::pack2(v[2] * f, v[3] * f);
+                        float2 v0, v1;
+                        w8_widen4(ws[h], v0, v1);
+                        v0 = fmul2(v0, f2(f));
+                        v1 = fmul2(v1, f2(f));
+                        o[2 * h] = D::pack2(v0.x, v0.y);
+                        o[2 * h + 1] = D::pack2(v1.x, v1.y);
                     }
                     // the two column blocks write their chunks in opposite order:
                     // 8 neighbouring lanes then touch all 8 chunks of a row
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         const int q = warp & 3;
         constexpr int COLS = BN / (D::EW / 4);
         const int col0 = ((warp - 2 - D::CW) >> 2) * COLS;
-        int64_t seg = 0;
+        RingPos<2> ra;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
@@ -394,10 +398,9 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 float sum[COLS];
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) sum[i] = 0.f;
-                for (int b = 0; b < nb; b += D::SEG, ++seg) {
-                    const int a = (int)(seg & 1);
-                    ok = ws_wait(&acc_full[a], (uint32_t)((seg / 2) & 1), abort, p.err);
-                    ok = __all_sync(0xffffffffu, ok);
+                for (int b = 0; b < nb; b += D::SEG, ra.next()) {
+                    const int a = ra.s;
+                    ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t trow =
@@ -418,11 +421,10 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) put(col0 + i, sum[i]);
             } else {
-                const int a = (int)(seg & 1);
-                ok = ws_wait(&acc_full[a], (uint32_t)((seg / 2) & 1), abort, p.err);
-                ok = __all_sync(0xffffffffu, ok);
+                const int a = ra.s;
+                ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
                 if (!ok) break;
-                ++seg;
+                ra.next();
                 tc_fence_after();
                 const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC);
 #pragma unroll 1
