@@ -18,14 +18,20 @@ such a checkpoint of the sum::
     z = kept * rstd;  g = dn * weight
     dx = dresidual = rstd * (g - z * mean(g * z)) + dh;   dweight = sum(dn * z)
 
+``weight_grad_ckpt`` forms a linear's weight gradient from what its input's
+checkpoint holds.  ``norm_linear_ckpt`` and ``linear_ckpt`` are the two layers
+built of them: the norm's and the linear's backward share one checkpoint.
+
 The reference has no counterpart: it keeps and multiplies everything in fp32.
 Sums, statistics and scales are fp32; results repeat bit for bit.
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -33,6 +39,12 @@ GROUP = 128        # columns of a checkpoint's group
 MAX_COLS = 16384   # widest row of the row kernels
 
 _TYPES = {torch.float32: _lib.MMB_F32, torch.bfloat16: _lib.MMB_BF16, torch.float16: _lib.MMB_F16}
+
+# A decoding step's kernels take a few microseconds, so its calls are held to a few
+# too: the raw stream handle (torch.cuda.current_stream() builds an object, 3 us), one
+# tensor for the small outputs of a call, sizes given one by one.
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_get_device = torch._C._cuda_getDevice
 
 
 def _type(t: torch.Tensor, what: str) -> int:
@@ -49,12 +61,25 @@ def _out_type(dtype: torch.dtype) -> int:
     return code
 
 
+def _index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The CUDA device that holds every given tensor; raises where there is none."""
+    idx = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != idx:
+            idx = -1
+    if idx < 0:
+        _lib.require_cuda(first, *others)
+    return idx
+
+
 def _rows2(t: torch.Tensor) -> torch.Tensor:
     """(rows, cols) with unit-stride rows that do not overlap."""
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1])
-    if (t.stride(1) != 1 and t.shape[1] != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
-        t = t.contiguous()
+        t = t.detach().reshape(-1, t.shape[-1])
+    s0, s1 = t.stride()
+    if (s1 != 1 or s0 < t.shape[1]) and ((s1 != 1 and t.shape[1] != 1)
+                                         or (t.shape[0] > 1 and s0 < t.shape[1])):
+        t = t.detach().contiguous()
     return t
 
 
@@ -65,21 +90,21 @@ def _ld(t: torch.Tensor) -> int:
 def _weight(weight: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]:
     if weight is None:
         return None
-    if weight.shape != (cols,):
+    if weight.dim() != 1 or weight.shape[0] != cols:
         raise ValueError(f"weight must be ({cols},), got {tuple(weight.shape)}")
-    weight = weight.detach()
-    if weight.dtype != torch.float32 or not weight.is_contiguous():
-        weight = weight.float().contiguous()
+    if weight.dtype != torch.float32 or weight.stride(0) != 1:
+        weight = weight.detach().float().contiguous()
     return weight
 
 
-def _call(name: str, on: torch.Tensor, *args) -> None:
+def _call(name: str, idx: int, *args) -> None:
+    """One library call on the current stream of device idx."""
     fn = getattr(_lib.load(), name)
-    if on.device.index == torch.cuda.current_device():
-        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if idx == _get_device():
+        st = fn(*args, _raw_stream(idx))
     else:
-        with torch.cuda.device(on.device):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(idx):
+            st = fn(*args, _raw_stream(idx))
     if st:
         _lib.check(st, name)
 
@@ -90,24 +115,25 @@ def _p(t: Optional[torch.Tensor]):
 
 def _empty_q(rows: int, cols: int, device) -> torch.Tensor:
     """int8 rows that start on 16-byte boundaries."""
-    pitch = (cols + 15) // 16 * 16
-    q = torch.empty((rows, pitch), dtype=torch.int8, device=device)
-    return q if pitch == cols else q[:, :cols]
+    return torch.empty_strided((rows, cols), ((cols + 15) // 16 * 16, 1), dtype=torch.int8,
+                               device=device)
 
 
-def _check_rows(x: torch.Tensor, residual: Optional[torch.Tensor], what: str):
+def _check_rows(x: torch.Tensor, residual: Optional[torch.Tensor], what: str) -> int:
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"{what}: x must have a last dimension of one or more")
-    if x.shape[-1] > MAX_COLS:
+    cols = x.shape[-1]
+    if cols > MAX_COLS:
         raise ValueError(f"{what}: rows of more than {MAX_COLS} values are not supported, "
-                         f"got {x.shape[-1]}")
+                         f"got {cols}")
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError(f"{what}: x and residual must share a shape, got {tuple(x.shape)} "
                              f"and {tuple(residual.shape)}")
-        if residual.dtype not in (x.dtype, torch.float32):
+        if residual.dtype != x.dtype and residual.dtype != torch.float32:
             raise ValueError(f"{what}: the residual must be of x's type or fp32, got "
                              f"{residual.dtype} with x {x.dtype}")
+    return cols
 
 
 class Q8Rows:
@@ -153,38 +179,37 @@ class Ckpt8:
 
 
 def _restore(q, scale, grouped, dtype):
-    _lib.require_cuda(q, scale)
+    idx = _index(q, scale)
     code = _out_type(dtype)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
     q2 = _rows2(q)
-    if out.numel():
+    rows, cols = q2.shape
+    if rows and cols:
         scale = scale.contiguous()
-        cols = q2.shape[1]
-        _call("mmb_restore_q8", q, q2.shape[0], cols, _p(q2), _ld(q2), _p(scale), int(grouped),
-              code, _p(out), cols)
+        _call("mmb_restore_q8", idx, rows, cols, q2.data_ptr(), _ld(q2), scale.data_ptr(), grouped,
+              code, out.data_ptr(), cols)
     return out
 
 
 def _norm_q8(x, weight, residual, eps, norm, what):
-    _lib.require_cuda(x, weight, residual)
-    xt = _type(x, what + ": x")
-    _check_rows(x, residual, what)
-    cols = x.shape[-1]
-    x2 = _rows2(x.detach())
+    idx = _index(x, weight, residual)
+    xt = rt = _type(x, what + ": x")
+    cols = _check_rows(x, residual, what)
+    weight = _weight(weight, cols)
+    x2, dev = _rows2(x), x.device
     rows = x2.shape[0]
-    w = _weight(weight, cols)
-    h = r2 = None
-    rt = xt
+    h = rp = hp = None
+    ldr = cols
     if residual is not None:
-        rt = _type(residual, what + ": residual")
-        r2 = _rows2(residual.detach())
-        h = torch.empty(x.shape, dtype=residual.dtype, device=x.device)
-    q = _empty_q(rows, cols, x.device)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        rt = _TYPES[residual.dtype]
+        r2 = _rows2(residual)
+        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        rp, hp, ldr = r2.data_ptr(), h.data_ptr(), _ld(r2)
+    q = _empty_q(rows, cols, dev)
+    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
     if rows:
-        _call("mmb_norm_q8", x, rows, cols, xt, _p(x2), _ld(x2), rt, _p(r2),
-              cols if r2 is None else _ld(r2), _p(w), eps, norm, _p(h), cols, _p(q), _ld(q),
-              _p(scale))
+        _call("mmb_norm_q8", idx, rows, cols, xt, x2.data_ptr(), _ld(x2), rt, rp, ldr, _p(weight),
+              eps, norm, hp, cols, q.data_ptr(), _ld(q), scale.data_ptr())
     if x.dim() != 2:
         q = q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0]
     return Q8Rows(q, scale), h
@@ -197,7 +222,7 @@ def rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     x (..., cols) fp32, bf16 or fp16; residual of x's shape, in x's type or
     fp32, None for none; weight (cols,) or None.  h is a new tensor in the
     residual's type (x itself without a residual).  No gradient."""
-    rows, h = _norm_q8(x, weight, residual, float(eps), 1, "rms_norm_q8")
+    rows, h = _norm_q8(x, weight, residual, eps, 1, "rms_norm_q8")
     return rows, x if h is None else h
 
 
@@ -208,12 +233,19 @@ def quantize_rows(x: torch.Tensor) -> Q8Rows:
 
 def _tma_rows(t: torch.Tensor) -> torch.Tensor:
     """int8 (rows, cols) whose rows start on 16-byte boundaries: t itself where they do."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and (
-            t.shape[0] == 1 or (t.stride(0) % 16 == 0 and t.stride(0) >= t.shape[1])):
+    rows, cols = t.shape
+    s0, s1 = t.stride()
+    if (s1 == 1 or cols == 1) and t.data_ptr() % 16 == 0 and (
+            rows == 1 or (s0 % 16 == 0 and s0 >= cols)):
         return t
-    out = _empty_q(t.shape[0], t.shape[1], t.device)
+    out = _empty_q(rows, cols, t.device)
     out.copy_(t)
     return out
+
+
+def _ld16(t: torch.Tensor) -> int:
+    """Row stride for the tensor maps: one row has whichever multiple of 16 holds it."""
+    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
 
 
 def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
@@ -223,8 +255,8 @@ def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
     Sums are exact integers (K <= 131071), scaled in fp32 and rounded once.
     Rows that do not start on 16-byte boundaries (quantize_rows and rms_norm_q8
     make ones that do) are copied first.  No gradient."""
-    xq, wq = x.q, w.q
-    _lib.require_cuda(xq, x.scale, wq, w.scale, bias)
+    xq, wq, xs, ws = x.q, w.q, x.scale, w.scale
+    idx = _index(xq, xs, wq, ws, bias)
     code = _out_type(out_dtype)
     if wq.dim() != 2 or xq.dim() < 1 or xq.shape[-1] != wq.shape[1]:
         raise ValueError(f"linear_q8: x (..., K) and w (N, K) must share K, got {tuple(xq.shape)} "
@@ -233,116 +265,121 @@ def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
     if not 1 <= K <= 131071 or N < 1:
         raise ValueError(f"linear_q8: K must be 1..131071 and N at least 1, got K {K}, N {N}")
     if bias is not None:
-        if bias.shape != (N,):
+        if bias.dim() != 1 or bias.shape[0] != N:
             raise ValueError(f"linear_q8: bias must be ({N},), got {tuple(bias.shape)}")
-        bias = bias.detach().float().contiguous()
-    out = torch.empty((*xq.shape[:-1], N), dtype=out_dtype, device=xq.device)
+        if bias.dtype != torch.float32 or bias.stride(0) != 1:
+            bias = bias.detach().float().contiguous()
+    out = torch.empty(*xq.shape[:-1], N, dtype=out_dtype, device=xq.device)
     if xq.dim() != 2:
         xq = xq.reshape(-1, K)
     M = xq.shape[0]
     if M:
-        xq, wq = _tma_rows(xq), _tma_rows(wq)
-        xs, ws = x.scale.contiguous(), w.scale.contiguous()
-        _call("mmb_gemm_q8", out, M, N, K, xq.data_ptr(), _ld16(xq), xs.data_ptr(), wq.data_ptr(),
+        xq, wq, xs, ws = _tma_rows(xq), _tma_rows(wq), xs.contiguous(), ws.contiguous()
+        _call("mmb_gemm_q8", idx, M, N, K, xq.data_ptr(), _ld16(xq), xs.data_ptr(), wq.data_ptr(),
               _ld16(wq), ws.data_ptr(), _p(bias), code, out.data_ptr(), N)
     return out
 
 
-def _ld16(t: torch.Tensor) -> int:
-    """Row stride for the tensor maps: one row has whichever multiple of 16 holds it."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
-
-
 def _norm_ckpt(x, weight, residual, eps, norm, n_dtype, keep, what):
-    """(n, h, q, scale, rstd) of one mmb_norm_ck8_fwd call; x and residual checked here."""
-    _lib.require_cuda(x, weight, residual)
-    xt = _type(x, what + ": x")
-    _check_rows(x, residual, what)
-    cols = x.shape[-1]
-    x2 = _rows2(x)
-    rows, dev = x2.shape[0], x.device
-    w = _weight(weight, cols)
-    h = r2 = n = q = scale = rstd = None
-    rt = xt
+    """(n, h, q, stats) of one mmb_norm_ck8_fwd call.  stats: the groups' scales and,
+    with norm, one rstd a row behind them, in one fp32 tensor."""
+    idx = _index(x, weight, residual)
+    xt = rt = _type(x, what + ": x")
+    cols = _check_rows(x, residual, what)
+    weight = _weight(weight, cols)
+    x2, dev = _rows2(x), x.device
+    rows = x2.shape[0]
+    h = n = q = stats = rp = hp = sp = vp = None
+    ldr = cols
     if residual is not None:
-        rt = _type(residual, what + ": residual")
+        rt = _TYPES[residual.dtype]
         r2 = _rows2(residual)
         h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
+        rp, hp, ldr = r2.data_ptr(), h.data_ptr(), _ld(r2)
     nt = 0
     if n_dtype is not None:
         nt = _out_type(n_dtype)
         n = torch.empty(x.shape, dtype=n_dtype, device=dev)
     if keep:
+        groups = -(-cols // GROUP)
         q = _empty_q(rows, cols, dev)
-        scale = torch.empty((rows, -(-cols // GROUP)), device=dev)
-        if norm:
-            rstd = torch.empty((rows,), device=dev)
+        stats = torch.empty(rows * (groups + norm), dtype=torch.float32, device=dev)
+        sp = stats.data_ptr()
+        vp = sp + 4 * rows * groups if norm else None
     if rows:
-        _call("mmb_norm_ck8_fwd", x, rows, cols, xt, _p(x2), _ld(x2), rt, _p(r2),
-              cols if r2 is None else _ld(r2), _p(w), eps, norm, _p(h), cols, nt, _p(n), cols,
-              _p(q), cols if q is None else _ld(q), _p(scale), _p(rstd))
-    return n, h, q, scale, rstd
+        _call("mmb_norm_ck8_fwd", idx, rows, cols, xt, x2.data_ptr(), _ld(x2), rt, rp, ldr,
+              _p(weight), eps, norm, hp, cols, nt, _p(n), cols, _p(q),
+              cols if q is None else _ld(q), sp, vp)
+    return n, h, q, stats
 
 
 def checkpoint_rows(x: torch.Tensor) -> Ckpt8:
     """x (..., cols) kept in 8 bits (fp32, bf16 or fp16 in)."""
-    _, _, q, scale, _ = _norm_ckpt(x.detach(), None, None, 0.0, 0, None, True, "checkpoint_rows")
-    return Ckpt8(q, scale, x.shape)
+    _, _, q, stats = _norm_ckpt(x, None, None, 0.0, 0, None, True, "checkpoint_rows")
+    return Ckpt8(q, stats.view(q.shape[0], -(-q.shape[1] // GROUP)), x.shape)
 
 
-def _norm_ckpt_bwd(dn, dh, weight, q, scale, rstd, shape, dx_dtype, want_dw):
-    """(dx, dweight): dn (..., cols); dh in dx_dtype or None."""
-    cols = shape[-1]
-    dn2 = _rows2(dn)
-    dh2 = None if dh is None else _rows2(dh)
-    rows, dev = dn2.shape[0], dn.device
-    w = _weight(weight, cols)
-    dx = torch.empty(shape, dtype=dx_dtype, device=dev)
-    dw = work = None
-    if want_dw:
-        dw = torch.empty((cols,), device=dev)
-        work = torch.empty((_lib.load().mmb_norm_ck8_bwd_work_floats(rows, cols),), device=dev)
-    _call("mmb_norm_ck8_bwd", dn, rows, cols, _TYPES[dn.dtype], _p(dn2), _ld(dn2),
-          _TYPES[dx_dtype], _p(dh2), cols if dh2 is None else _ld(dh2), _p(w), _p(q), _ld(q),
-          _p(scale), _p(rstd), _p(dx), cols, _p(dw), _p(work))
-    return dx, dw
+@lru_cache(maxsize=256)
+def _bwd_floats(rows: int, cols: int) -> int:
+    return _lib.load().mmb_norm_ck8_bwd_work_floats(rows, cols)
 
 
-def _bwd_types(dn, dh, out_dtype):
-    """The types the backward kernel takes: dx in dn's type or fp32."""
+@lru_cache(maxsize=256)
+def _wgrad_floats(M: int, N: int, K: int, code: int) -> int:
+    return _lib.load().mmb_wgrad_ck8_work_floats(M, N, K, code)
+
+
+def _norm_ckpt_bwd(dn, dh, weight, q, stats, shape, out_dtype, want_dw):
+    """(dx, dweight) from dn (..., cols): dx in out_dtype or, where the kernel has no
+    such pair of types, fp32."""
+    rows, cols = q.shape
+    dev = dn.device
+    idx = _index(dn, dh, weight, q)
     dx_dtype = dn.dtype if out_dtype == dn.dtype else torch.float32
     if dh is not None and dh.dtype != dx_dtype:
         dh = dh.to(dx_dtype)
-    return dh, dx_dtype
+    dn2 = _rows2(dn)
+    dh2 = None if dh is None else _rows2(dh)
+    dx = torch.empty(shape, dtype=dx_dtype, device=dev)
+    dw = work = None
+    if want_dw:
+        dw = torch.empty(cols, dtype=torch.float32, device=dev)
+        work = torch.empty(_bwd_floats(rows, cols), dtype=torch.float32, device=dev)
+    sp = stats.data_ptr()
+    _call("mmb_norm_ck8_bwd", idx, rows, cols, _TYPES[dn.dtype], dn2.data_ptr(), _ld(dn2),
+          _TYPES[dx_dtype], _p(dh2), cols if dh2 is None else _ld(dh2),
+          _p(_weight(weight, cols)), q.data_ptr(), _ld(q), sp, sp + 4 * rows * -(-cols // GROUP),
+          dx.data_ptr(), cols, _p(dw), _p(work))
+    return dx, dw
+
+
+def _as(t: Optional[torch.Tensor], dtype) -> Optional[torch.Tensor]:
+    return t if t is None or t.dtype == dtype else t.to(dtype)
 
 
 class RmsNormCkptFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, n_dtype):
-        keep = any(ctx.needs_input_grad[:3])
-        n, h, q, scale, rstd = _norm_ckpt(x, weight, residual, eps, 1, n_dtype, keep,
-                                          "rms_norm_ckpt")
-        ctx.save_for_backward(weight, q, scale, rstd)
+        n, h, q, stats = _norm_ckpt(x, weight, residual, eps, 1, n_dtype,
+                                    any(ctx.needs_input_grad[:3]), "rms_norm_ckpt")
+        ctx.save_for_backward(weight, q, stats)
         ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         return (n, h) if h is not None else n
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dn, dh=None):
-        weight, q, scale, rstd = ctx.saved_tensors
         shape, xdt, rdt = ctx.meta
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
+        weight, q, stats = ctx.saved_tensors
         dw = None
         if dn is None:
             dx = dh
         else:
-            dh, dx_dtype = _bwd_types(dn, dh, rdt or xdt)
-            dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, scale, rstd, shape, dx_dtype,
-                                    need_w and weight is not None)
-        cast = lambda t, dt: None if t is None else t if t.dtype == dt else t.to(dt)
-        return (cast(dx, xdt) if need_x else None,
-                cast(dw, weight.dtype) if dw is not None else None,
-                cast(dx, rdt) if need_r and rdt is not None else None, None, None)
+            dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, stats, shape, rdt or xdt, need_w)
+        return (_as(dx, xdt) if need_x else None, None if dw is None else _as(dw, weight.dtype),
+                _as(dx, rdt) if need_r else None, None, None)
 
 
 def rms_norm_ckpt(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -354,7 +391,7 @@ def rms_norm_ckpt(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     Arguments as in rms_norm_q8; n is in out_dtype (x's type by default), h in
     the residual's type (x itself without a residual)."""
-    out = RmsNormCkptFn.apply(x, weight, residual, float(eps), out_dtype or x.dtype)
+    out = RmsNormCkptFn.apply(x, weight, residual, eps, out_dtype or x.dtype)
     return out if residual is not None else (out, x)
 
 
@@ -365,9 +402,9 @@ def _tma_grad(dy: torch.Tensor) -> torch.Tensor:
     if dy.data_ptr() % 16 == 0 and (dy.shape[0] == 1 or dy.stride(0) * size % 16 == 0):
         return dy
     unit = 16 // size
-    out = torch.empty((dy.shape[0], (dy.shape[1] + unit - 1) // unit * unit), dtype=dy.dtype,
-                      device=dy.device)[:, : dy.shape[1]]
-    out.copy_(dy)
+    out = torch.empty_strided(dy.shape, ((dy.shape[1] + unit - 1) // unit * unit, 1),
+                              dtype=dy.dtype, device=dy.device)
+    out.copy_(dy.detach())
     return out
 
 
@@ -376,7 +413,23 @@ def _factor(t: Optional[torch.Tensor], n: int, what: str) -> Optional[torch.Tens
         return None
     if t.numel() != n:
         raise ValueError(f"weight_grad_ckpt: {what} must hold {n} values, got {tuple(t.shape)}")
-    return t.detach().reshape(-1).float().contiguous()
+    if t.dtype != torch.float32 or not t.is_contiguous():
+        t = t.detach().float().contiguous()
+    return t
+
+
+def _weight_grad(idx, dy, code, q, scale_ptr, row_ptr, col_ptr, out_dtype, oc):
+    M, K = q.shape
+    N = dy.shape[-1]
+    dw = torch.empty(N, K, dtype=out_dtype, device=dy.device)
+    dy2, q = _tma_grad(dy), _tma_rows(q)
+    floats = _wgrad_floats(M, N, K, code)
+    work = torch.empty(floats, dtype=torch.float32, device=dy.device) if floats else None
+    unit = 16 // dy.element_size()
+    _call("mmb_wgrad_ck8", idx, M, N, K, code, dy2.data_ptr(),
+          dy2.stride(0) if M > 1 else -(-N // unit) * unit, q.data_ptr(), _ld16(q), scale_ptr,
+          row_ptr, col_ptr, oc, dw.data_ptr(), K, _p(work))
+    return dw
 
 
 def weight_grad_ckpt(dy: torch.Tensor, kept: Ckpt8, row_scale: Optional[torch.Tensor] = None,
@@ -389,24 +442,124 @@ def weight_grad_ckpt(dy: torch.Tensor, kept: Ckpt8, row_scale: Optional[torch.Te
     dy (..., N) fp32, bf16 or fp16 with kept's rows; row_scale (one a row) and
     col_scale (K,) are a norm's rstd and weight where the linear stands behind
     one.  In dy's type unless out_dtype says otherwise; sums are fp32."""
-    _lib.require_cuda(dy, kept.q, kept.scale, row_scale, col_scale)
+    q, scale = kept.q, kept.scale
+    idx = _index(dy, q, scale, row_scale, col_scale)
     code = _type(dy, "weight_grad_ckpt: dy")
-    M, K = kept.q.shape
+    M, K = q.shape
     if dy.dim() < 1 or dy.shape[-1] < 1 or dy.numel() != M * dy.shape[-1]:
         raise ValueError(f"weight_grad_ckpt: dy (..., N) must have the checkpoint's {M} rows, got "
                          f"{tuple(dy.shape)}")
-    N = dy.shape[-1]
     row, col = _factor(row_scale, M, "row_scale"), _factor(col_scale, K, "col_scale")
     out_dtype = out_dtype or dy.dtype
-    oc = _out_type(out_dtype)
-    dw = torch.empty((N, K), dtype=out_dtype, device=dy.device)
-    dy2, q = _tma_grad(dy.detach()), _tma_rows(kept.q)
-    work = None
-    floats = _lib.load().mmb_wgrad_ck8_work_floats(M, N, K, code)
-    if floats:
-        work = torch.empty((floats,), device=dy.device)
-    unit = 16 // dy.element_size()
-    _call("mmb_wgrad_ck8", dy, M, N, K, code, dy2.data_ptr(),
-          dy2.stride(0) if M > 1 else -(-N // unit) * unit, q.data_ptr(), _ld16(q),
-          kept.scale.data_ptr(), _p(row), _p(col), oc, dw.data_ptr(), K, _p(work))
-    return dw
+    return _weight_grad(idx, dy, code, q, scale.data_ptr(), _p(row), _p(col), out_dtype,
+                        _out_type(out_dtype))
+
+
+def _linear_types(x_dtype: torch.dtype) -> torch.dtype:
+    """The type a linear's product runs in: autocast's where it is on, else x's."""
+    if torch.is_autocast_enabled("cuda"):
+        return torch.get_autocast_dtype("cuda")
+    return x_dtype
+
+
+def _linear(n, weight, bias):
+    dt = n.dtype
+    with torch.autocast("cuda", enabled=False):
+        return torch.nn.functional.linear(n, weight.to(dt), None if bias is None else bias.to(dt))
+
+
+class NormLinearCkptFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, norm_weight, residual, weight, bias, eps):
+        dt = _linear_types(weight.dtype)
+        n, h, q, stats = _norm_ckpt(x, norm_weight, residual, eps, 1, dt,
+                                    any(ctx.needs_input_grad[:5]), "norm_linear_ckpt")
+        y = _linear(n, weight, bias)
+        ctx.save_for_backward(norm_weight, weight, q, stats)
+        ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype,
+                    None if bias is None else bias.dtype)
+        ctx.set_materialize_grads(False)
+        return (y, h) if h is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        shape, xdt, rdt, bdt = ctx.meta
+        need = ctx.needs_input_grad
+        norm_weight, weight, q, stats = ctx.saved_tensors
+        if dy is None:
+            return _as(dh, xdt), None, _as(dh, rdt) if need[2] else None, None, None, None
+        rows, cols = q.shape
+        dx = dnw = dw = db = None
+        if need[0] or need[1] or need[2]:
+            with torch.autocast("cuda", enabled=False):
+                dn = torch.matmul(dy, weight.to(dy.dtype))
+            dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, shape, rdt or xdt, need[1])
+        if need[3]:
+            sp, nw = stats.data_ptr(), _weight(norm_weight, cols)
+            dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, sp,
+                              sp + 4 * rows * -(-cols // GROUP), _p(nw), weight.dtype,
+                              _out_type(weight.dtype))
+        if need[4] and bdt is not None:
+            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
+        return (_as(dx, xdt) if need[0] else None,
+                None if dnw is None else _as(dnw, norm_weight.dtype),
+                _as(dx, rdt) if need[2] else None, dw, db, None)
+
+
+def norm_linear_ckpt(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weight: torch.Tensor,
+                     bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                     eps: float = 1e-5):
+    """(y, h): y = linear(rms_norm(h), weight, bias) of h = x + residual, and h.
+
+    One 8-bit checkpoint of h serves both backward passes, the norm's and the
+    weight's; neither h nor the norm is kept.  The product runs in the weight's
+    type (autocast's where it is on); weight is (N, cols) fp32, bf16 or fp16."""
+    _linear_check(x, weight, bias, "norm_linear_ckpt")
+    out = NormLinearCkptFn.apply(x, norm_weight, residual, weight, bias, eps)
+    return out if residual is not None else (out, x)
+
+
+class LinearCkptFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        q = stats = None
+        if ctx.needs_input_grad[1]:
+            _, _, q, stats = _norm_ckpt(x, None, None, 0.0, 0, None, True, "linear_ckpt")
+        ctx.save_for_backward(weight, q, stats)
+        ctx.meta = (x.dtype, None if bias is None else bias.dtype)
+        return _linear(x.to(_linear_types(weight.dtype)), weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        xdt, bdt = ctx.meta
+        need = ctx.needs_input_grad
+        weight, q, stats = ctx.saved_tensors
+        dx = dw = db = None
+        if need[0]:
+            with torch.autocast("cuda", enabled=False):
+                dx = _as(torch.matmul(dy, weight.to(dy.dtype)), xdt)
+        if need[1]:
+            dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, stats.data_ptr(), None,
+                              None, weight.dtype, _out_type(weight.dtype))
+        if need[2] and bdt is not None:
+            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
+        return dx, dw, db
+
+
+def linear_ckpt(x: torch.Tensor, weight: torch.Tensor,
+                bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """linear(x, weight, bias) that keeps x in 8 bits for the weight's gradient."""
+    _linear_check(x, weight, bias, "linear_ckpt")
+    return LinearCkptFn.apply(x, weight, bias)
+
+
+def _linear_check(x, weight, bias, what):
+    _lib.require_cuda(x, weight, bias)
+    _type(weight, what + ": weight")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: x (..., K) and weight (N, K) must share K, got {tuple(x.shape)} "
+                         f"and {tuple(weight.shape)}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != weight.shape[0]):
+        raise ValueError(f"{what}: bias must be ({weight.shape[0]},), got {tuple(bias.shape)}")
