@@ -56,12 +56,12 @@ struct G8Params {
     const float* bias;  // nullable
     void* out;
     int64_t ldo;
-    int tma_out;  // out goes through TMA boxes (16-byte aligned rows)
-    int vec_cols; // ws and bias take 16-byte loads
+    int out_align;  // bytes every row of out starts on a multiple of: 32, 16 or less
+    int vec_cols;   // ws and bias take 16-byte loads
     int* err;
 };
 struct G8Maps {
-    CUtensorMap x, w, out;
+    CUtensorMap x, w;
 };
 
 template <int OT>
@@ -90,34 +90,64 @@ struct G8Out<MMB_F16> {
     }
 };
 
-__device__ __forceinline__ void tma_store_box(const CUtensorMap* map, const void* src, int c0,
-                                              int c1) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group"
-        " [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
-        "r"(c0), "r"(c1), "r"(0), "r"(smem_u32(src))
-        : "memory");
+// 32 bytes at once (sm_100): whole sectors, so rows need no staging
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
+                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+// 32 neighbouring values of a row, in its type
+template <int OT>
+__device__ __forceinline__ void g8_store32(typename G8Out<OT>::T* p, const float (&v)[32],
+                                           int align, int valid) {
+    using O = G8Out<OT>;
+    constexpr int WORDS = OT == MMB_F32 ? 32 : 16;
+    if (valid >= 32 && align >= 16) {
+        uint32_t w[WORDS];
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (OT == MMB_F32) w[i] = __float_as_uint(v[i]);
+            else w[i] = O::pack2(v[2 * i], v[2 * i + 1]);
+        }
+        uint32_t* d = reinterpret_cast<uint32_t*>(p);
+        if (align >= 32) {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 8) {
+                const uint32_t t[8] = {w[i],     w[i + 1], w[i + 2], w[i + 3],
+                                       w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
+                st_global_32(d + i, t);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < WORDS; i += 4)
+                *reinterpret_cast<uint4*>(d + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < valid) p[i] = O::from_f(v[i]);
+    }
 }
 
 // ---------------------------------------------------------------------------
 // tiles
 // ---------------------------------------------------------------------------
-constexpr int G8_NT = 32 * 6;
+constexpr int G8_EW = 8;  // epilogue warps: two per TMEM lane quarter, half of the columns each
+constexpr int G8_NT = 32 * (2 + G8_EW);
 constexpr int G8_GROUP_M = 16;  // tiles of a group share their weights' panels in L2
 template <int BN>
 __host__ __device__ constexpr int g8_ring() { return BN == 256 ? 4 : 6; }
 template <int BN>
 struct G8Smem {
     static constexpr int A = G8_BM * G8_BK, B = BN * G8_BK, SLOT = A + B;
-    static constexpr int EPI = 4 * 2 * 4096;  // two 4 KB boxes per epilogue warp
-    static constexpr size_t BYTES = (size_t)g8_ring<BN>() * SLOT + EPI + 1024;
+    static constexpr size_t BYTES = (size_t)g8_ring<BN>() * SLOT + 1024;
 };
 
 template <int BN, int OT>
 __global__ void __launch_bounds__(G8_NT, 1)
     g8_tile_kernel(const G8Params p, const __grid_constant__ G8Maps maps) {
     using Sm = G8Smem<BN>;
-    using O = G8Out<OT>;
+    using T = typename G8Out<OT>::T;
     constexpr int R = g8_ring<BN>();
     constexpr uint32_t IDESC = i8_idesc(BN);
     extern __shared__ float4 g8_smem4[];
@@ -127,7 +157,6 @@ __global__ void __launch_bounds__(G8_NT, 1)
     volatile int* abort = &abort_s;
     char* smem = reinterpret_cast<char*>(
         (reinterpret_cast<uintptr_t>(g8_smem4) + 1023) & ~(uintptr_t)1023);
-    char* epi = smem + R * Sm::SLOT;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
     const int64_t mt = (p.M + G8_BM - 1) / G8_BM, nt = (p.N + BN - 1) / BN;
@@ -149,7 +178,7 @@ __global__ void __launch_bounds__(G8_NT, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&acc_full[a], 1);
-            mbar_init(&acc_empty[a], 128);
+            mbar_init(&acc_empty[a], 32 * G8_EW);
         }
         mbar_init(&drained, 1);
         mbar_fence_init();
@@ -163,19 +192,19 @@ __global__ void __launch_bounds__(G8_NT, 1)
     if (warp == 0) {
         // ---- producer ----
         if (lane == 0) {
+            RingPos<R> r;
             int64_t j = 0;
             bool ok = true;
             for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x) {
                 int64_t m0, n0;
                 tile_of(t, m0, n0);
-                for (int k = 0; k < nk; ++k, ++j) {
-                    const int s = (int)(j % R);
-                    if (j >= R) ok = ws_wait(&empty[s], (uint32_t)(((j / R) - 1) & 1), abort, p.err);
+                for (int k = 0; k < nk; ++k, ++j, r.next()) {
+                    ok = ws_wait(&empty[r.s], r.ph ^ 1u, abort, p.err);
                     if (!ok) break;
-                    char* slot = smem + s * Sm::SLOT;
-                    mbar_expect_tx(&full[s], Sm::SLOT);
-                    tma_load_3d(slot, &maps.x, k * G8_BK, (int)m0, 0, &full[s]);
-                    tma_load_3d(slot + Sm::A, &maps.w, k * G8_BK, (int)n0, 0, &full[s]);
+                    char* slot = smem + r.s * Sm::SLOT;
+                    mbar_expect_tx(&full[r.s], Sm::SLOT);
+                    tma_load_3d(slot, &maps.x, k * G8_BK, (int)m0, 0, &full[r.s]);
+                    tma_load_3d(slot + Sm::A, &maps.w, k * G8_BK, (int)n0, 0, &full[r.s]);
                 }
             }
             // copies still in flight land before the CTA leaves
@@ -185,136 +214,86 @@ __global__ void __launch_bounds__(G8_NT, 1)
     } else if (warp == 1) {
         // ---- MMA issuer ----
         if (lane == 0) {
-            int64_t j = 0, lt = 0;
+            RingPos<R> r;
+            RingPos<2> ra;
             bool ok = true;
-            for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++lt) {
-                const int a = (int)(lt & 1);
-                if (lt >= 2) ok = ws_wait(&acc_empty[a], (uint32_t)(((lt / 2) - 1) & 1), abort, p.err);
+            for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ra.next()) {
+                ok = ws_wait(&acc_empty[ra.s], ra.ph ^ 1u, abort, p.err);
                 if (!ok) break;
                 tc_fence_after();
-                const uint32_t acc = tmem + (uint32_t)(a * BN);
-                for (int k = 0; k < nk; ++k, ++j) {
-                    const int s = (int)(j % R);
-                    ok = ws_wait(&full[s], (uint32_t)((j / R) & 1), abort, p.err);
+                const uint32_t acc = tmem + (uint32_t)(ra.s * BN);
+                for (int k = 0; k < nk; ++k, r.next()) {
+                    ok = ws_wait(&full[r.s], r.ph, abort, p.err);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(smem + s * Sm::SLOT);
+                    const uint32_t sa = smem_u32(smem + r.s * Sm::SLOT);
 #pragma unroll
                     for (int kk = 0; kk < G8_BK / 32; ++kk)
                         umma_i8(acc, g8_desc(sa, kk), g8_desc(sa + Sm::A, kk), IDESC,
                                 (k > 0 || kk > 0) ? 1u : 0u);
-                    umma_commit(&empty[s]);
+                    umma_commit(&empty[r.s]);
                 }
-                if (ok) umma_commit(&acc_full[a]);
+                if (ok) umma_commit(&acc_full[ra.s]);
             }
             // every MMA this CTA issued has completed before TMEM is freed
             umma_commit(&drained);
             mbar_wait_polls(&drained, 0, 1 << 20);
         }
     } else {
-        // ---- epilogue: warp q = warp % 4 reads TMEM lanes 32q..32q+31 ----
-        const int q = warp & 3;
-        char* wb = epi + q * 2 * 4096;
-        int64_t lt = 0;
-        int nbox = 0;
-        bool ok = true;
-        for (int64_t t = blockIdx.x; t < ntiles && ok; t += gridDim.x, ++lt) {
+        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (tokens) 32q..32q+31; a lane
+        // stores 32 columns of its token at a time, whole 32-byte sectors ----
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        RingPos<2> ra;
+        for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ra.next()) {
             int64_t m0, n0;
             tile_of(t, m0, n0);
-            const int a = (int)(lt & 1);
             const int64_t m = m0 + q * 32 + lane;
             const float sx = m < p.M ? p.xs[m] : 0.f;
-            ok = ws_wait(&acc_full[a], (uint32_t)((lt / 2) & 1), abort, p.err);
-            if (!ok) break;
-            tc_fence_after();
             const int ncols = (int)min64(p.N - n0, BN);
-            const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * BN);
-            uint32_t rr[2][32];
-            tmem_ld32_issue(trow, rr[0]);
-            tmem_wait32(rr[0]);
-#pragma unroll
-            for (int c = 0; c < BN; c += 32) {
-                const int cur = (c >> 5) & 1;
-                if (c >= ncols) continue;
-                if (c + 32 < ncols) tmem_ld32_issue(trow + (uint32_t)(c + 32), rr[cur ^ 1]);
+            if (!__all_sync(0xffffffffu, ws_wait(&acc_full[ra.s], ra.ph, abort, p.err))) break;
+            tc_fence_after();
+            const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ra.s * BN);
+#pragma unroll 1
+            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && c < ncols; c += 32) {
+                uint32_t r[32];
+                tmem_ld32_issue(trow + (uint32_t)c, r);
                 const int64_t nb = n0 + c;
-                float v[32];
-                if (p.vec_cols && c + 32 <= ncols) {
+                float w[32], v[32];
+                const bool whole = p.vec_cols && c + 32 <= ncols;
+                if (whole) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
                         const float4 w4 = *reinterpret_cast<const float4*>(p.ws + nb + j);
-                        v[j] = (float)(int)rr[cur][j] * sx * w4.x;
-                        v[j + 1] = (float)(int)rr[cur][j + 1] * sx * w4.y;
-                        v[j + 2] = (float)(int)rr[cur][j + 2] * sx * w4.z;
-                        v[j + 3] = (float)(int)rr[cur][j + 3] * sx * w4.w;
-                    }
-                    if (p.bias) {
-#pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            const float4 b4 = *reinterpret_cast<const float4*>(p.bias + nb + j);
-                            v[j] += b4.x;
-                            v[j + 1] += b4.y;
-                            v[j + 2] += b4.z;
-                            v[j + 3] += b4.w;
-                        }
+                        w[j] = w4.x; w[j + 1] = w4.y; w[j + 2] = w4.z; w[j + 3] = w4.w;
                     }
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        v[j] = 0.f;
-                        if (c + j < ncols) {
-                            v[j] = (float)(int)rr[cur][j] * sx * p.ws[nb + j];
-                            if (p.bias) v[j] += p.bias[nb + j];
-                        }
-                    }
+                    for (int j = 0; j < 32; ++j) w[j] = c + j < ncols ? p.ws[nb + j] : 0.f;
                 }
-                if (p.tma_out) {
-                    // 32 rows x 128 bytes a box: 32 fp32 columns, or two chunks of 16-bit ones
-                    constexpr bool WIDE = OT == MMB_F32;
-                    const int half = WIDE ? 0 : cur;
-                    char* buf = wb + (nbox & 1) * 4096;
-                    if (half == 0) {
-                        if (lane == 0) bulk_wait_read<1>();  // what this buffer held has left
-                        __syncwarp();
-                    }
-                    if constexpr (WIDE) {
+                tmem_wait32(r);
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            reinterpret_cast<float4*>(buf + lane * 128)[j ^ (lane & 7)] =
-                                make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+                for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * sx * w[j];
+                if (p.bias) {
+                    if (whole) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            const float4 b4 = *reinterpret_cast<const float4*>(p.bias + nb + j);
+                            v[j] += b4.x; v[j + 1] += b4.y; v[j + 2] += b4.z; v[j + 3] += b4.w;
+                        }
                     } else {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            reinterpret_cast<uint4*>(buf + lane * 128)[(half * 4 + j) ^ (lane & 7)] =
-                                make_uint4(O::pack2(v[8 * j], v[8 * j + 1]),
-                                           O::pack2(v[8 * j + 2], v[8 * j + 3]),
-                                           O::pack2(v[8 * j + 4], v[8 * j + 5]),
-                                           O::pack2(v[8 * j + 6], v[8 * j + 7]));
+                        for (int j = 0; j < 32; ++j)
+                            if (c + j < ncols) v[j] += p.bias[nb + j];
                     }
-                    if (WIDE || half == 1 || c + 32 >= ncols) {
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (lane == 0) {
-                            tma_store_box(&maps.out, buf, (int)(nb - (half ? 32 : 0)),
-                                          (int)(m0 + q * 32));
-                            bulk_commit();
-                        }
-                        ++nbox;
-                    }
-                } else if (m < p.M) {
-                    typename O::T* orow = static_cast<typename O::T*>(p.out) + m * p.ldo + nb;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        if (c + j < ncols) orow[j] = O::from_f(v[j]);
                 }
+                if (m < p.M)
+                    g8_store32<OT>(static_cast<T*>(p.out) + m * p.ldo + nb, v, p.out_align,
+                                   ncols - c);
                 __syncwarp();
-                if (c + 32 < ncols) tmem_wait32(rr[cur ^ 1]);
             }
             tc_fence_before();
-            mbar_arrive(&acc_empty[a]);
+            mbar_arrive(&acc_empty[ra.s]);
         }
-        if (lane == 0) bulk_wait_read<0>();
-        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -339,15 +318,18 @@ struct G8SSmem {
     static_assert(RING >= MT * 128 * 4, "the ring's space holds the partial sums");
 };
 __device__ __forceinline__ void cluster_sync() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\n\t"
                  "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ int ld_cluster(uint32_t saddr, uint32_t rank) {
-    int v;
+// 4 values from another CTA of the cluster (volatile: the loads stay between the
+// cluster barriers, but nothing waits for one before the next is issued)
+__device__ __forceinline__ int4 ld_cluster4(uint32_t saddr, uint32_t rank) {
+    int4 v;
     asm volatile("{\n\t.reg .b32 a;\n\t"
-                 "mapa.shared::cluster.u32 a, %1, %2;\n\t"
-                 "ld.shared::cluster.s32 %0, [a];\n\t}"
-                 : "=r"(v) : "r"(saddr), "r"(rank) : "memory");
+                 "mapa.shared::cluster.u32 a, %4, %5;\n\t"
+                 "ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [a];\n\t}"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(saddr), "r"(rank));
     return v;
 }
 
@@ -430,7 +412,6 @@ __global__ void __launch_bounds__(G8S_NT, 1)
     // partial sums, token-major: part[j][channel]
     int* part = reinterpret_cast<int*>(smem);
     const int ch = tid;  // TMEM lane = channel of the tile
-    const int64_t n = n0 + ch;
     if (nk > 0) {
 #pragma unroll
         for (int c = 0; c < TC; c += 32) {
@@ -445,23 +426,35 @@ __global__ void __launch_bounds__(G8S_NT, 1)
     tc_fence_before();
     if (splits > 1) cluster_sync();
     else __syncthreads();
-    const float sw = n < p.N ? p.ws[n] : 0.f;
-    const float sb = n < p.N && p.bias ? p.bias[n] : 0.f;
-    // each rank finishes its share of the tokens
-    for (int j = rank; j < MT; j += splits) {
-        const int64_t m = m0 + j;
-        if (m >= p.M) break;
-        int acc = 0;
+    // each rank finishes its share of the tokens, 4 channels a thread
+    const int share = (MT + splits - 1 - rank) / splits;
+    for (int i = tid; i < share * 32; i += G8S_NT) {
+        const int j = (i >> 5) * splits + rank, c = (i & 31) * 4;
+        const int64_t m = m0 + j, n = n0 + c;
+        if (m >= p.M || n >= p.N) continue;
+        int4 t = make_int4(0, 0, 0, 0);
         if (splits == 1) {
-            acc = part[j * 128 + ch];
+            t = *reinterpret_cast<const int4*>(part + j * 128 + c);
         } else {
-            const uint32_t a = smem_u32(part + j * 128 + ch);
-            for (int r = 0; r < active; ++r) acc += ld_cluster(a, (uint32_t)r);
+            const uint32_t a = smem_u32(part + j * 128 + c);
+            int4 v[G8S_MAX_SPLIT];
+#pragma unroll
+            for (int r = 0; r < G8S_MAX_SPLIT; ++r)
+                v[r] = r < active ? ld_cluster4(a, (uint32_t)r) : make_int4(0, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < G8S_MAX_SPLIT; ++r) {
+                t.x += v[r].x; t.y += v[r].y; t.z += v[r].z; t.w += v[r].w;
+            }
         }
-        if (n < p.N) {
-            float v = (float)acc * p.xs[m] * sw;
-            if (p.bias) v += sb;
-            static_cast<typename O::T*>(p.out)[m * p.ldo + n] = O::from_f(v);
+        const float sx = p.xs[m];
+        const int acc[4] = {t.x, t.y, t.z, t.w};
+        typename O::T* o = static_cast<typename O::T*>(p.out) + m * p.ldo + n;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (n + e >= p.N) break;
+            float v = (float)acc[e] * sx * p.ws[n + e];
+            if (p.bias) v += p.bias[n + e];
+            o[e] = O::from_f(v);
         }
     }
     if (splits > 1) cluster_sync();  // no CTA leaves while its sums are being read
@@ -475,17 +468,12 @@ __global__ void __launch_bounds__(G8S_NT, 1)
 // host side
 // ---------------------------------------------------------------------------
 template <int BN, int OT>
-static int g8_tile_launch(const G8Params& p0, const int8_t* x, int64_t ldx, const int8_t* w,
+static int g8_tile_launch(const G8Params& p, const int8_t* x, int64_t ldx, const int8_t* w,
                           int64_t ldw, cudaStream_t s) {
-    G8Params p = p0;
     G8Maps maps;
     if (!mmb_encode_tile_map(&maps.x, x, 1, p.K, p.M, 1, ldx, ldx * p.M, G8_BK, G8_BM, 128) ||
         !mmb_encode_tile_map(&maps.w, w, 1, p.K, p.N, 1, ldw, ldw * p.N, G8_BK, BN, 128))
         return MMB_ERR_ALIGN;
-    constexpr int OB = OT == MMB_F32 ? 4 : 2;
-    p.tma_out = ((uintptr_t)p.out & 15) == 0 && (p.ldo * OB) % 16 == 0 &&
-                mmb_encode_tile_map(&maps.out, p.out, OB, p.N, p.M, 1, p.ldo, p.ldo * p.M,
-                                    128 / OB, 32, 128);
     static int attr[MMB_MAX_DEVICES] = {};
     const int st = mmb_smem_attr(g8_tile_kernel<BN, OT>, G8Smem<BN>::BYTES, attr);
     if (st != MMB_OK) return st;
@@ -569,6 +557,8 @@ extern "C" int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int
     p.M = M; p.N = N; p.K = K;
     p.xs = xs; p.ws = ws; p.bias = bias; p.out = out; p.ldo = ldo;
     p.vec_cols = ((uintptr_t)ws & 15) == 0 && ((uintptr_t)bias & 15) == 0;
+    const uintptr_t rows = (uintptr_t)out | (uintptr_t)(ldo * (out_type == MMB_F32 ? 4 : 2));
+    p.out_align = rows % 32 == 0 ? 32 : rows % 16 == 0 ? 16 : 1;
     p.err = mmb_device_error_flag();
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (out_type == MMB_F32) return g8_dispatch<MMB_F32>(p, x, ldx, w, ldw, s);

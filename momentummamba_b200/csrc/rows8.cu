@@ -446,86 +446,99 @@ struct R8Bwd {
     float* part;  // gridDim.x x cols partial sums of dweight (null: none wanted)
 };
 
-// Blocks walk rows (blockDim.y at a time) and keep their columns' share of
-// dweight in registers; at the end a block's rows-in-flight are added up in
-// shared memory and the block writes its own line of partial sums, which
-// r8_colsum_kernel adds in a fixed order: the result does not depend on timing.
-template <class EN, class EX, bool VEC, int NC, int NT>
+// Blocks walk rows, blockDim.y * U at a time: a warp loads U rows at once (narrow
+// rows leave too few bytes in flight otherwise: 32768 x 128 fp32 took 24 us with
+// one row a warp).  Each thread keeps its columns' share of dweight in
+// registers; at the end a block's rows-in-flight are added up in shared memory
+// and the block writes its own line of partial sums, which r8_colsum_kernel adds
+// in a fixed order: the result does not depend on timing.
+template <class EN, class EX, bool VEC, int NC, int U, int NT>
 __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
     extern __shared__ float r8_acc[];  // blockDim.y x cols, when blockDim.y > 1
     __shared__ float2 part[R8_MAX_WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
     const int64_t groups = (p.cols + R8_GROUP - 1) / R8_GROUP;
     const auto col0 = [&](int c) { return (int64_t)(c * nw + warp) * R8_CHUNK; };
+    const int64_t step = (int64_t)gridDim.x * blockDim.y;
+    constexpr int G = VEC ? 1 : 2;  // groups a lane's 8 values fall into
     float acc[NC][8];
 #pragma unroll
     for (int c = 0; c < NC; ++c)
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[c][j] = 0.f;
 
-    for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows;
-         row += (int64_t)gridDim.x * blockDim.y) {
-        const auto* dnr = static_cast<const typename EN::T*>(p.dn) + row * p.dns;
-        R8Load<EN, VEC> ln[NC];
-        R8LoadQ<VEC> lq[NC];
-        float s[NC][VEC ? 1 : 2];
+    for (int64_t row0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row0 < p.rows;
+         row0 += step * U) {
+        R8Load<EN, VEC> ln[U][NC];
+        R8Load<EX, VEC> lh[U][NC];
+        R8LoadQ<VEC> lq[U][NC];
+        float s[U][NC][G], rstd[U];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) ln[c].load(dnr, col0(c), lane, p.cols);
+        for (int u = 0; u < U; ++u) {
+            // a row past the end loads the last one again and stores nothing
+            const int64_t row = min64(row0 + u * step, p.rows - 1);
+            const auto* dnr = static_cast<const typename EN::T*>(p.dn) + row * p.dns;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            lq[c].load(p.q + row * p.qs, col0(c), lane, p.cols);
+            for (int c = 0; c < NC; ++c) ln[u][c].load(dnr, col0(c), lane, p.cols);
+            if (p.dh) {
+                const auto* dhr = static_cast<const typename EX::T*>(p.dh) + row * p.dhs;
 #pragma unroll
-            for (int g = 0; g < (VEC ? 1 : 2); ++g) {
-                const int64_t gc = col0(c) + (VEC ? (lane >> 4) : g) * R8_GROUP;
-                s[c][g] = gc < p.cols ? p.scale[row * groups + gc / R8_GROUP] : 0.f;
+                for (int c = 0; c < NC; ++c) lh[u][c].load(dhr, col0(c), lane, p.cols);
             }
-        }
-        const float rstd = p.rstd[row];
-        float z[NC][8], g[NC][8], dot = 0.f;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            lq[c].get(z[c]);
-            ln[c].get(g[c]);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                z[c][j] *= s[c][VEC ? 0 : j >> 2] * rstd;
-                acc[c][j] = fmaf(g[c][j], z[c][j], acc[c][j]);
-            }
-            if (p.w) {
-                R8Load<T8F32, VEC> lw;
-                float w[8];
-                lw.load(p.w, col0(c), lane, p.cols);
-                lw.get(w);
-#pragma unroll
-                for (int j = 0; j < 8; ++j) g[c][j] *= w[j];
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dot = fmaf(g[c][j], z[c][j], dot);
-        }
-        float unused = 0.f;
-        r8_row_reduce(dot, unused, part);
-        const float mean = __fdiv_rn(dot, (float)p.cols);
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) g[c][j] = rstd * fmaf(-z[c][j], mean, g[c][j]);
-        if (p.dh) {
-            const auto* dhr = static_cast<const typename EX::T*>(p.dh) + row * p.dhs;
-            R8Load<EX, VEC> lh[NC];
-#pragma unroll
-            for (int c = 0; c < NC; ++c) lh[c].load(dhr, col0(c), lane, p.cols);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
-                float a[8];
-                lh[c].get(a);
+                lq[u][c].load(p.q + row * p.qs, col0(c), lane, p.cols);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) g[c][j] += a[j];
+                for (int g = 0; g < G; ++g) {
+                    const int64_t gc = col0(c) + (VEC ? (lane >> 4) : g) * R8_GROUP;
+                    s[u][c][g] = gc < p.cols ? p.scale[row * groups + gc / R8_GROUP] : 0.f;
+                }
             }
+            rstd[u] = p.rstd[row];
         }
-        auto* dxr = static_cast<typename EX::T*>(p.dx) + row * p.dxs;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) r8_store<EX, VEC>(dxr, col0(c), lane, p.cols, g[c]);
-        if (nw > 1) __syncthreads();  // `part` is written again for the next row
+        for (int u = 0; u < U; ++u) {
+            const int64_t row = row0 + u * step;
+            if (row >= p.rows) break;  // the same for a whole warp, and for a block of one row
+            float z[NC][8], g[NC][8], dot = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                lq[u][c].get(z[c]);
+                ln[u][c].get(g[c]);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    z[c][j] *= s[u][c][VEC ? 0 : j >> 2] * rstd[u];
+                    acc[c][j] = fmaf(g[c][j], z[c][j], acc[c][j]);
+                }
+                if (p.w) {
+                    R8Load<T8F32, VEC> lw;
+                    float w[8];
+                    lw.load(p.w, col0(c), lane, p.cols);
+                    lw.get(w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[c][j] *= w[j];
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) dot = fmaf(g[c][j], z[c][j], dot);
+            }
+            float unused = 0.f;
+            r8_row_reduce(dot, unused, part);
+            const float mean = __fdiv_rn(dot, (float)p.cols);
+            auto* dxr = static_cast<typename EX::T*>(p.dx) + row * p.dxs;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) g[c][j] = rstd[u] * fmaf(-z[c][j], mean, g[c][j]);
+                if (p.dh) {
+                    float a[8];
+                    lh[u][c].get(a);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) g[c][j] += a[j];
+                }
+                r8_store<EX, VEC>(dxr, col0(c), lane, p.cols, g[c]);
+            }
+            if (nw > 1) __syncthreads();  // `part` is written again for the next row
+        }
     }
     if (!p.part) return;
     float* out = p.part + (int64_t)blockIdx.x * p.cols;
@@ -557,54 +570,60 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
 }
 
 // out[k] = sum of the lines' column k, in a fixed order
-constexpr int R8_SUM_ROWS = 8;
-__global__ void __launch_bounds__(32 * R8_SUM_ROWS)
+constexpr int R8_SUM_ROWS = 32, R8_SUM_COLS = 32;
+__global__ void __launch_bounds__(R8_SUM_COLS* R8_SUM_ROWS)
     r8_colsum_kernel(const float* __restrict__ part, int lines, int64_t cols,
                      float* __restrict__ out) {
-    __shared__ float s[R8_SUM_ROWS][32];
-    const int64_t k = (int64_t)blockIdx.x * 32 + threadIdx.x;
+    __shared__ float s[R8_SUM_ROWS][R8_SUM_COLS];
+    const int64_t k = (int64_t)blockIdx.x * R8_SUM_COLS + threadIdx.x;
     float t = 0.f;
-    if (k < cols)
+    if (k < cols) {
+#pragma unroll 8
         for (int l = threadIdx.y; l < lines; l += R8_SUM_ROWS) t += part[(int64_t)l * cols + k];
+    }
     s[threadIdx.y][threadIdx.x] = t;
     __syncthreads();
-    if (threadIdx.y == 0 && k < cols) {
 #pragma unroll
-        for (int r = 1; r < R8_SUM_ROWS; ++r) t += s[r][threadIdx.x];
-        out[k] = t;
+    for (int h = R8_SUM_ROWS / 2; h >= 1; h >>= 1) {
+        if (threadIdx.y < h) s[threadIdx.y][threadIdx.x] += s[threadIdx.y + h][threadIdx.x];
+        __syncthreads();
     }
+    if (threadIdx.y == 0 && k < cols) out[k] = s[0][threadIdx.x];
 }
 
-// Restored rows: q * scale (one per row, or one per group of 128 columns).
+// Restored rows: q * scale (one per row, or one per group of 128 columns).  A
+// warp takes 256 columns of R8_RROWS rows, all loads first.
+constexpr int R8_RROWS = 4;
 template <class E, bool VEC>
 __global__ void __launch_bounds__(256)
     r8_restore_kernel(int64_t rows, int64_t cols, const int8_t* __restrict__ q, int64_t qs,
                       const float* __restrict__ scale, int64_t groups, void* out, int64_t os) {
     const int lane = threadIdx.x & 31;
-    const int64_t chunks = (cols + R8_CHUNK - 1) / R8_CHUNK;
-    const int64_t u = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int64_t row = u / chunks, c0 = (u % chunks) * R8_CHUNK;
-    if (row >= rows) return;
-    R8LoadQ<VEC> lq;
-    lq.load(q + row * qs, c0, lane, cols);
-    float v[8];
-    lq.get(v);
-    if constexpr (VEC) {
-        const int64_t gc = c0 + (lane >> 4) * R8_GROUP;
-        const float s = groups ? (gc < cols ? scale[row * groups + gc / R8_GROUP] : 0.f) : scale[row];
+    const int64_t c0 = (int64_t)blockIdx.y * R8_CHUNK;
+    const int64_t row0 = ((int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5)) * R8_RROWS;
+    if (row0 >= rows) return;
+    constexpr int G = VEC ? 1 : 2;
+    R8LoadQ<VEC> lq[R8_RROWS];
+    float s[R8_RROWS][G];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= s;
-    } else {
+    for (int i = 0; i < R8_RROWS; ++i) {
+        const int64_t row = min64(row0 + i, rows - 1);
+        lq[i].load(q + row * qs, c0, lane, cols);
 #pragma unroll
-        for (int g = 0; g < 2; ++g) {
-            const int64_t gc = c0 + g * R8_GROUP;
-            const float s =
-                groups ? (gc < cols ? scale[row * groups + gc / R8_GROUP] : 0.f) : scale[row];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[4 * g + j] *= s;
+        for (int g = 0; g < G; ++g) {
+            const int64_t gc = c0 + (VEC ? (lane >> 4) : g) * R8_GROUP;
+            s[i][g] = !groups ? scale[row] : gc < cols ? scale[row * groups + gc / R8_GROUP] : 0.f;
         }
     }
-    r8_store<E, VEC>(static_cast<typename E::T*>(out) + row * os, c0, lane, cols, v);
+#pragma unroll
+    for (int i = 0; i < R8_RROWS; ++i) {
+        if (row0 + i >= rows) break;
+        float v[8];
+        lq[i].get(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= s[i][VEC ? 0 : j >> 2];
+        r8_store<E, VEC>(static_cast<typename E::T*>(out) + (row0 + i) * os, c0, lane, cols, v);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -619,9 +638,11 @@ static R8Shape r8_shape(int64_t cols) {
     if (chunks <= 1) return {1, 1, 4};
     if (chunks <= 2) return {1, 2, 4};
     if (chunks <= 4) return {1, 4, 4};
-    const int64_t warps = (chunks + 3) / 4;
-    if (warps > R8_MAX_WARPS) return {0, 0, 0};
-    return {(int)warps, 4, 1};
+    // several warps a row: two chunks each as long as 16 warps suffice (four leave
+    // a 512-thread block too few registers)
+    if (chunks <= 2 * R8_MAX_WARPS) return {(int)((chunks + 1) / 2), 2, 1};
+    if (chunks <= 4 * R8_MAX_WARPS) return {(int)((chunks + 3) / 4), 4, 1};
+    return {0, 0, 0};
 }
 static int r8_bytes(int dt) { return dt == MMB_F32 ? 4 : 2; }
 static bool r8_type(int dt) { return dt == MMB_F32 || dt == MMB_BF16 || dt == MMB_F16; }
@@ -638,7 +659,9 @@ static int r8_fwd_launch(const R8Fwd& p, const R8Shape& s, cudaStream_t st) {
     const dim3 block(32 * s.warps, s.rows);
     const unsigned grid = (unsigned)((p.rows + s.rows - 1) / s.rows);
     if (s.nc == 1) r8_fwd_kernel<EX, ER, VEC, 1, 128, CK><<<grid, block, 0, st>>>(p);
-    else if (s.nc == 2) r8_fwd_kernel<EX, ER, VEC, 2, 128, CK><<<grid, block, 0, st>>>(p);
+    else if (s.nc == 2 && s.warps == 1)
+        r8_fwd_kernel<EX, ER, VEC, 2, 128, CK><<<grid, block, 0, st>>>(p);
+    else if (s.nc == 2) r8_fwd_kernel<EX, ER, VEC, 2, 512, CK><<<grid, block, 0, st>>>(p);
     else if (s.warps == 1) r8_fwd_kernel<EX, ER, VEC, 4, 128, CK><<<grid, block, 0, st>>>(p);
     else r8_fwd_kernel<EX, ER, VEC, 4, 512, CK><<<grid, block, 0, st>>>(p);
     return mmb_launch_status();
@@ -687,10 +710,12 @@ template <class EN, class EX, bool VEC>
 static int r8_bwd_launch(const R8Bwd& p, const R8Shape& s, int blocks, cudaStream_t st) {
     const dim3 block(32 * s.warps, s.rows);
     const size_t sm = s.rows > 1 ? (size_t)s.rows * p.cols * sizeof(float) : 0;  // <= 16 KB
-    if (s.nc == 1) r8_bwd_kernel<EN, EX, VEC, 1, 128><<<blocks, block, sm, st>>>(p);
-    else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, 128><<<blocks, block, sm, st>>>(p);
-    else if (s.warps == 1) r8_bwd_kernel<EN, EX, VEC, 4, 128><<<blocks, block, sm, st>>>(p);
-    else r8_bwd_kernel<EN, EX, VEC, 4, 512><<<blocks, block, sm, st>>>(p);
+    if (s.nc == 1) r8_bwd_kernel<EN, EX, VEC, 1, 4, 128><<<blocks, block, sm, st>>>(p);
+    else if (s.nc == 2 && s.warps == 1)
+        r8_bwd_kernel<EN, EX, VEC, 2, 2, 128><<<blocks, block, sm, st>>>(p);
+    else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, 1, 512><<<blocks, block, sm, st>>>(p);
+    else if (s.warps == 1) r8_bwd_kernel<EN, EX, VEC, 4, 1, 128><<<blocks, block, sm, st>>>(p);
+    else r8_bwd_kernel<EN, EX, VEC, 4, 1, 512><<<blocks, block, sm, st>>>(p);
     return mmb_launch_status();
 }
 
@@ -772,7 +797,8 @@ extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, con
     else rc = dx_type == MMB_F32 ? R8_BWD(T8F16, T8F32) : R8_BWD(T8F16, T8F16);
 #undef R8_BWD
     if (rc != MMB_OK || !dweight) return rc;
-    r8_colsum_kernel<<<(unsigned)((cols + 31) / 32), dim3(32, R8_SUM_ROWS), 0, st>>>(
+    r8_colsum_kernel<<<(unsigned)((cols + R8_SUM_COLS - 1) / R8_SUM_COLS),
+                       dim3(R8_SUM_COLS, R8_SUM_ROWS), 0, st>>>(
         work, blocks, cols, dweight);
     return mmb_launch_status();
 }
@@ -787,19 +813,19 @@ extern "C" int mmb_restore_q8(int64_t rows, int64_t cols, const int8_t* q, int64
     if (!q || !scale || !out) return MMB_ERR_NULL;
     if (ldq < cols || ldo < cols) return MMB_ERR_SHAPE;
     const int64_t chunks = (cols + R8_CHUNK - 1) / R8_CHUNK;
-    const int64_t blocks = (rows * chunks + 7) / 8;
-    if (blocks > INT32_MAX) return MMB_ERR_SHAPE;
+    if (chunks > 65535) return MMB_ERR_UNSUPPORTED;
+    const dim3 blocks((unsigned)((rows + 8 * R8_RROWS - 1) / (8 * R8_RROWS)), (unsigned)chunks);
     const int64_t groups = grouped ? (cols + R8_GROUP - 1) / R8_GROUP : 0;
     const bool vec = cols % 8 == 0 && r8_aligned(out, ldo, r8_bytes(out_type)) && r8_aligned_q(q, ldq);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
 #define R8_RESTORE(E)                                                                           \
     do {                                                                                        \
         if (vec)                                                                                \
-            r8_restore_kernel<E, true><<<(unsigned)blocks, 256, 0, st>>>(rows, cols, q, ldq, scale, \
-                                                                         groups, out, ldo);     \
+            r8_restore_kernel<E, true><<<blocks, 256, 0, st>>>(rows, cols, q, ldq, scale,       \
+                                                               groups, out, ldo);               \
         else                                                                                    \
-            r8_restore_kernel<E, false><<<(unsigned)blocks, 256, 0, st>>>(rows, cols, q, ldq,   \
-                                                                          scale, groups, out, ldo); \
+            r8_restore_kernel<E, false><<<blocks, 256, 0, st>>>(rows, cols, q, ldq, scale,      \
+                                                                groups, out, ldo);              \
     } while (0)
     if (out_type == MMB_F32) R8_RESTORE(T8F32);
     else if (out_type == MMB_BF16) R8_RESTORE(T8BF16);
