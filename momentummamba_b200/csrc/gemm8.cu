@@ -56,12 +56,11 @@ struct G8Params {
     const float* bias;  // nullable
     void* out;
     int64_t ldo;
-    int out_align;  // bytes every row of out starts on a multiple of: 32, 16 or less
-    int vec_cols;   // ws and bias take 16-byte loads
+    int tma_out;  // out goes through TMA boxes (16-byte aligned rows)
     int* err;
 };
 struct G8Maps {
-    CUtensorMap x, w;
+    CUtensorMap x, w, out;
 };
 
 template <int OT>
@@ -90,43 +89,13 @@ struct G8Out<MMB_F16> {
     }
 };
 
-// 32 bytes at once (sm_100): whole sectors, so rows need no staging
-__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]),
-                 "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
-                 : "memory");
-}
-// 32 neighbouring values of a row, in its type
-template <int OT>
-__device__ __forceinline__ void g8_store32(typename G8Out<OT>::T* p, const float (&v)[32],
-                                           int align, int valid) {
-    using O = G8Out<OT>;
-    constexpr int WORDS = OT == MMB_F32 ? 32 : 16;
-    if (valid >= 32 && align >= 16) {
-        uint32_t w[WORDS];
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            if constexpr (OT == MMB_F32) w[i] = __float_as_uint(v[i]);
-            else w[i] = O::pack2(v[2 * i], v[2 * i + 1]);
-        }
-        uint32_t* d = reinterpret_cast<uint32_t*>(p);
-        if (align >= 32) {
-#pragma unroll
-            for (int i = 0; i < WORDS; i += 8) {
-                const uint32_t t[8] = {w[i],     w[i + 1], w[i + 2], w[i + 3],
-                                       w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
-                st_global_32(d + i, t);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < WORDS; i += 4)
-                *reinterpret_cast<uint4*>(d + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < valid) p[i] = O::from_f(v[i]);
-    }
+__device__ __forceinline__ void tma_store_box(const CUtensorMap* map, const void* src, int c0,
+                                              int c1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group"
+        " [%0, {%1, %2, %3}], [%4];" ::"l"(reinterpret_cast<uint64_t>(map)),
+        "r"(c0), "r"(c1), "r"(0), "r"(smem_u32(src))
+        : "memory");
 }
 
 // ---------------------------------------------------------------------------
@@ -140,24 +109,32 @@ __host__ __device__ constexpr int g8_ring() { return BN == 256 ? 4 : 6; }
 template <int BN>
 struct G8Smem {
     static constexpr int A = G8_BM * G8_BK, B = BN * G8_BK, SLOT = A + B;
-    static constexpr size_t BYTES = (size_t)g8_ring<BN>() * SLOT + 1024;
+    static constexpr int EPI = G8_EW * 4096;  // a 4 KB box per epilogue warp
+    static constexpr size_t BYTES = (size_t)g8_ring<BN>() * SLOT + EPI;
 };
 
 template <int BN, int OT>
 __global__ void __launch_bounds__(G8_NT, 1)
     g8_tile_kernel(const G8Params p, const __grid_constant__ G8Maps maps) {
     using Sm = G8Smem<BN>;
-    using T = typename G8Out<OT>::T;
+    using O = G8Out<OT>;
+    using T = typename O::T;
     constexpr int R = g8_ring<BN>();
     constexpr uint32_t IDESC = i8_idesc(BN);
-    extern __shared__ float4 g8_smem4[];
+    // 1024-byte aligned: no room to round up (227 KB with the static part)
+    extern __shared__ __align__(1024) char g8_smem[];
     __shared__ uint64_t full[R], empty[R], acc_full[2], acc_empty[2], drained;
+    __shared__ float4 chan4[2][BN / 4];  // a tile's channel scales and biases
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
+    float(*chan)[BN] = reinterpret_cast<float(*)[BN]>(chan4);
     volatile int* abort = &abort_s;
-    char* smem = reinterpret_cast<char*>(
-        (reinterpret_cast<uintptr_t>(g8_smem4) + 1023) & ~(uintptr_t)1023);
+    char* smem = g8_smem;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    if (smem_u32(smem) & 1023u) {
+        if (tid == 0 && p.err) atomicOr(p.err, 1);
+        return;
+    }
 
     const int64_t mt = (p.M + G8_BM - 1) / G8_BM, nt = (p.N + BN - 1) / BN;
     const int64_t ntiles = mt * nt;
@@ -240,60 +217,115 @@ __global__ void __launch_bounds__(G8_NT, 1)
             mbar_wait_polls(&drained, 0, 1 << 20);
         }
     } else {
-        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (tokens) 32q..32q+31; a lane
-        // stores 32 columns of its token at a time, whole 32-byte sectors ----
-        const int q = warp & 3, half = (warp - 2) >> 2;
+        // ---- epilogue: warp q = warp % 4 reads TMEM lanes (tokens) 32q..32q+31; 32
+        // columns at a time go through a box in shared memory to a TMA store.  The scales
+        // and the bias of a tile are loaded one tile ahead, the channels' through shared
+        // memory ----
+        const int q = warp & 3, half = (warp - 2) >> 2, et = tid - 64;
+        constexpr int PER = BN / 2;  // columns of a warp
+        char* box = smem + R * Sm::SLOT + (warp - 2) * 4096;
         RingPos<2> ra;
-        for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ra.next()) {
-            int64_t m0, n0;
+        int64_t m0, n0;
+        float sx = 0.f, wn = 0.f, bn = 0.f;
+        const auto ahead = [&](int64_t t) {
+            if (t >= ntiles) return;
             tile_of(t, m0, n0);
-            const int64_t m = m0 + q * 32 + lane;
-            const float sx = m < p.M ? p.xs[m] : 0.f;
+            const int64_t m = m0 + q * 32 + lane, n = n0 + et;
+            sx = m < p.M ? p.xs[m] : 0.f;
+            if (et < BN && n < p.N) {
+                wn = p.ws[n];
+                if (p.bias) bn = p.bias[n];
+            }
+        };
+        ahead(blockIdx.x);
+        for (int64_t t = blockIdx.x; t < ntiles; t += gridDim.x, ra.next()) {
+            const int64_t m = m0 + q * 32 + lane, nt0 = n0;
             const int ncols = (int)min64(p.N - n0, BN);
-            if (!__all_sync(0xffffffffu, ws_wait(&acc_full[ra.s], ra.ph, abort, p.err))) break;
+            const float sm = sx;
+            // the sums are there, and every warp is done with the channels' values of the
+            // tile before; a wait that gave up ends the role for all of its warps at once
+            if (!bar_and<1, 32 * G8_EW>(ws_wait(&acc_full[ra.s], ra.ph, abort, p.err))) break;
             tc_fence_after();
-            const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ra.s * BN);
-#pragma unroll 1
-            for (int c = half * (BN / 2); c < (half + 1) * (BN / 2) && c < ncols; c += 32) {
-                uint32_t r[32];
-                tmem_ld32_issue(trow + (uint32_t)c, r);
-                const int64_t nb = n0 + c;
-                float w[32], v[32];
-                const bool whole = p.vec_cols && c + 32 <= ncols;
-                if (whole) {
+            if (et < BN) {
+                chan[0][et] = wn;
+                chan[1][et] = bn;
+            }
+            ahead(t + gridDim.x);
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * G8_EW) : "memory");
+            const uint32_t trow =
+                tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(ra.s * BN + half * PER);
+            uint32_t r[2][32];
+            tmem_ld32_issue(trow, r[0]);
+            tmem_wait32(r[0]);
+#pragma unroll
+            for (int c = 0; c < PER; c += 32) {
+                const int cur = (c >> 5) & 1, col = half * PER + c;
+                if (c + 32 < PER) tmem_ld32_issue(trow + (uint32_t)(c + 32), r[cur ^ 1]);
+                if (col < ncols) {
+                    float v[32];
 #pragma unroll
                     for (int j = 0; j < 32; j += 4) {
-                        const float4 w4 = *reinterpret_cast<const float4*>(p.ws + nb + j);
-                        w[j] = w4.x; w[j + 1] = w4.y; w[j + 2] = w4.z; w[j + 3] = w4.w;
+                        const float4 w4 = *reinterpret_cast<const float4*>(&chan[0][col + j]);
+                        v[j] = (float)(int)r[cur][j] * sm * w4.x;
+                        v[j + 1] = (float)(int)r[cur][j + 1] * sm * w4.y;
+                        v[j + 2] = (float)(int)r[cur][j + 2] * sm * w4.z;
+                        v[j + 3] = (float)(int)r[cur][j + 3] * sm * w4.w;
                     }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) w[j] = c + j < ncols ? p.ws[nb + j] : 0.f;
-                }
-                tmem_wait32(r);
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = (float)(int)r[j] * sx * w[j];
-                if (p.bias) {
-                    if (whole) {
+                    if (p.bias) {
 #pragma unroll
                         for (int j = 0; j < 32; j += 4) {
-                            const float4 b4 = *reinterpret_cast<const float4*>(p.bias + nb + j);
+                            const float4 b4 = *reinterpret_cast<const float4*>(&chan[1][col + j]);
                             v[j] += b4.x; v[j + 1] += b4.y; v[j + 2] += b4.z; v[j + 3] += b4.w;
                         }
-                    } else {
+                    }
+                    if (p.tma_out) {
+                        // 32 tokens x 128 bytes a box: 32 fp32 columns, or two chunks of 16-bit ones
+                        constexpr bool WIDE = OT == MMB_F32;
+                        const int part = WIDE ? 0 : cur;
+                        if (part == 0) {
+                            if (lane == 0) bulk_wait_read<0>();  // the box before has left
+                            __syncwarp();
+                        }
+                        uint4* row = reinterpret_cast<uint4*>(box + lane * 128);
+                        if constexpr (WIDE) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j)
+                                row[j ^ (lane & 7)] = make_uint4(
+                                    __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                    __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 4; ++j)
+                                row[(part * 4 + j) ^ (lane & 7)] = make_uint4(
+                                    O::pack2(v[8 * j], v[8 * j + 1]),
+                                    O::pack2(v[8 * j + 2], v[8 * j + 3]),
+                                    O::pack2(v[8 * j + 4], v[8 * j + 5]),
+                                    O::pack2(v[8 * j + 6], v[8 * j + 7]));
+                        }
+                        if (WIDE || part == 1 || col + 32 >= ncols) {
+                            fence_proxy_async_smem();
+                            __syncwarp();
+                            if (lane == 0) {
+                                tma_store_box(&maps.out, box, (int)nt0 + col - (part ? 32 : 0),
+                                              (int)m - lane);
+                                bulk_commit();
+                            }
+                        }
+                    } else if (m < p.M) {
+                        T* o = static_cast<T*>(p.out) + m * p.ldo + nt0 + col;
 #pragma unroll
                         for (int j = 0; j < 32; ++j)
-                            if (c + j < ncols) v[j] += p.bias[nb + j];
+                            if (col + j < ncols) o[j] = O::from_f(v[j]);
                     }
                 }
-                if (m < p.M)
-                    g8_store32<OT>(static_cast<T*>(p.out) + m * p.ldo + nb, v, p.out_align,
-                                   ncols - c);
                 __syncwarp();
+                if (c + 32 < PER) tmem_wait32(r[cur ^ 1]);
             }
             tc_fence_before();
             mbar_arrive(&acc_empty[ra.s]);
         }
+        if (lane == 0) bulk_wait_read<0>();
+        __syncwarp();
     }
     tc_fence_before();
     __syncthreads();
@@ -468,12 +500,17 @@ __global__ void __launch_bounds__(G8S_NT, 1)
 // host side
 // ---------------------------------------------------------------------------
 template <int BN, int OT>
-static int g8_tile_launch(const G8Params& p, const int8_t* x, int64_t ldx, const int8_t* w,
+static int g8_tile_launch(const G8Params& p0, const int8_t* x, int64_t ldx, const int8_t* w,
                           int64_t ldw, cudaStream_t s) {
+    G8Params p = p0;
     G8Maps maps;
     if (!mmb_encode_tile_map(&maps.x, x, 1, p.K, p.M, 1, ldx, ldx * p.M, G8_BK, G8_BM, 128) ||
         !mmb_encode_tile_map(&maps.w, w, 1, p.K, p.N, 1, ldw, ldw * p.N, G8_BK, BN, 128))
         return MMB_ERR_ALIGN;
+    constexpr int OB = OT == MMB_F32 ? 4 : 2;
+    p.tma_out = ((uintptr_t)p.out & 15) == 0 && (p.ldo * OB) % 16 == 0 &&
+                mmb_encode_tile_map(&maps.out, p.out, OB, p.N, p.M, 1, p.ldo, p.ldo * p.M,
+                                    128 / OB, 32, 128);
     static int attr[MMB_MAX_DEVICES] = {};
     const int st = mmb_smem_attr(g8_tile_kernel<BN, OT>, G8Smem<BN>::BYTES, attr);
     if (st != MMB_OK) return st;
@@ -556,9 +593,6 @@ extern "C" int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int
     G8Params p{};
     p.M = M; p.N = N; p.K = K;
     p.xs = xs; p.ws = ws; p.bias = bias; p.out = out; p.ldo = ldo;
-    p.vec_cols = ((uintptr_t)ws & 15) == 0 && ((uintptr_t)bias & 15) == 0;
-    const uintptr_t rows = (uintptr_t)out | (uintptr_t)(ldo * (out_type == MMB_F32 ? 4 : 2));
-    p.out_align = rows % 32 == 0 ? 32 : rows % 16 == 0 ? 16 : 1;
     p.err = mmb_device_error_flag();
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (out_type == MMB_F32) return g8_dispatch<MMB_F32>(p, x, ldx, w, ldw, s);

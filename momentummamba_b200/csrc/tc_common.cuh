@@ -129,6 +129,22 @@ __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
+// Barrier `ID` over THREADS threads of the CTA: true on all of them when `ok` was.
+template <int ID, int THREADS>
+__device__ __forceinline__ bool bar_and(bool ok) {
+    uint32_t all;
+    __syncwarp();
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, %2, %3, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(all)
+        : "r"((uint32_t)ok), "n"(ID), "n"(THREADS)
+        : "memory");
+    return all != 0;
+}
+
 // A place in a ring of R slots and the phase of its barriers.  The side that
 // fills waits for the opposite phase: a fresh barrier counts as having passed
 // the phase before its first.
