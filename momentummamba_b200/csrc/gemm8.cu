@@ -340,8 +340,11 @@ __global__ void __launch_bounds__(G8_NT, 1)
 // ---------------------------------------------------------------------------
 constexpr int G8S_NT = 128;
 constexpr int G8S_MAX_SPLIT = 8;
+// Two CTAs share an SM (at most 108 KB each): a cluster of 8 then needs 4 SMs of a
+// GPC, where 8 whole ones often are not free at once (48 x 2048 x 4096: 16 clusters
+// of 8 ran in two waves, 12.5 us, of 4 in one, 8.1 us).
 template <int MT>
-__host__ __device__ constexpr int g8s_ring() { return MT <= 32 ? 10 : MT == 64 ? 8 : 6; }
+__host__ __device__ constexpr int g8s_ring() { return MT == 16 ? 6 : MT == 32 ? 5 : MT == 64 ? 4 : 3; }
 template <int MT>
 struct G8SSmem {
     static constexpr int W = 128 * G8_BK, X = MT * G8_BK, SLOT = W + X;
@@ -367,7 +370,7 @@ __device__ __forceinline__ int4 ld_cluster4(uint32_t saddr, uint32_t rank) {
 
 // grid (splits, channel tiles, token tiles), cluster (splits, 1, 1)
 template <int MT, int OT>
-__global__ void __launch_bounds__(G8S_NT, 1)
+__global__ void __launch_bounds__(G8S_NT, 2)
     g8_split_kernel(const G8Params p, const __grid_constant__ G8Maps maps) {
     using Sm = G8SSmem<MT>;
     using O = G8Out<OT>;
@@ -389,6 +392,13 @@ __global__ void __launch_bounds__(G8S_NT, 1)
     const int nk = ke > kb ? ke - kb : 0;
     const int active = (nkb + per - 1) / per;  // ranks that have K blocks
 
+    const auto load = [&](int j) {
+        char* slot = smem + (j % R) * Sm::SLOT;
+        uint64_t* bar = &full[j % R];
+        mbar_expect_tx(bar, Sm::SLOT);
+        tma_load_3d(slot, &maps.w, (kb + j) * G8_BK, (int)n0, 0, bar);
+        tma_load_3d(slot + Sm::W, &maps.x, (kb + j) * G8_BK, (int)m0, 0, bar);
+    };
     if (tid == 0) {
         abort_s = 0;
         for (int s = 0; s < R; ++s) {
@@ -397,6 +407,8 @@ __global__ void __launch_bounds__(G8S_NT, 1)
         }
         mbar_init(&done, 1);
         mbar_fence_init();
+        // the first loads need nothing but the barriers
+        for (int j = 0; j < nk && j < R; ++j) load(j);
     }
     if (warp == 1) tmem_alloc(&tmem_base_s, TC);
     tc_fence_before();
@@ -405,16 +417,10 @@ __global__ void __launch_bounds__(G8S_NT, 1)
     const uint32_t tmem = tmem_base_s;
 
     if (tid == 0) {
-        bool ok = true;
-        int j = 0;
+        int j = nk < R ? nk : R;
         for (; j < nk; ++j) {
-            const int s = j % R;
-            if (j >= R) ok = ws_wait(&empty[s], (uint32_t)(((j / R) - 1) & 1), abort, p.err);
-            if (!ok) break;
-            char* slot = smem + s * Sm::SLOT;
-            mbar_expect_tx(&full[s], Sm::SLOT);
-            tma_load_3d(slot, &maps.w, (kb + j) * G8_BK, (int)n0, 0, &full[s]);
-            tma_load_3d(slot + Sm::W, &maps.x, (kb + j) * G8_BK, (int)m0, 0, &full[s]);
+            if (!ws_wait(&empty[j % R], (uint32_t)(((j / R) - 1) & 1), abort, p.err)) break;
+            load(j);
         }
         for (int q = j - R > 0 ? j - R : 0; q < j; ++q)
             mbar_wait_polls(&full[q % R], (uint32_t)((q / R) & 1), 1 << 16);
@@ -532,9 +538,11 @@ static int g8_split_launch(const G8Params& p, const int8_t* x, int64_t ldx, cons
     if (st != MMB_OK) return st;
     const int64_t nt = (p.N + 127) / 128, mt = (p.M + MT - 1) / MT;
     const int nkb = (int)((p.K + G8_BK - 1) / G8_BK);
-    // as many K slices as leave no SM two CTAs, at least one K block each
+    // as many K slices as fit two CTAs an SM, at least two K blocks each (one token,
+    // 4096 x 1024: 8 slices of one block 5.5 us, 4 of two 4.6 us)
     int splits = 1;
-    while (splits < G8S_MAX_SPLIT && splits * 2 <= nkb && nt * mt * splits * 2 <= 148) splits *= 2;
+    while (splits < G8S_MAX_SPLIT && splits * 4 <= nkb && nt * mt * splits * 2 <= 2 * 148)
+        splits *= 2;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)splits, (unsigned)nt, (unsigned)mt);
     cfg.blockDim = dim3(G8S_NT);
