@@ -18,8 +18,8 @@
 //   * fp32 dy (times row, in fp32) is split into three bf16 parts, 24 bits in
 //     all, and multiplied with the exact q * s in three MMAs.
 //
-// Tile: 128 columns of the checkpoint (one group: a token has one scale) as the
-// MMA's rows, BN columns of dy as its columns, both "MN-major" (a token's
+// Tile: one or two groups of 128 checkpoint columns (a token has one scale in
+// each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a token's
 // values are contiguous; tokens are the reduction).  The tokens are cut into
 // slices so that tiles x slices fill the GPU; a slice's tile goes to a
 // workspace and w8_sum_kernel adds the slices in a fixed order.  Persistent,
@@ -63,25 +63,28 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
     return (uint32_t)(block * (BT * 128) + t * 128 + ((c ^ (t & 7)) << 4));
 }
 
-// BN: dy columns of a tile; BT: tokens of a block; RL, RC: blocks in flight as
-// they lie in memory / widened; CW, EW: converter and epilogue warps; SEG: token
-// blocks that accumulate in TMEM before the sums move to registers.
-struct W8BF16 {
-    static constexpr bool BF16 = true, F32 = false;
-    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 8, EW = 4, BYTES = 2;
-    static constexpr int SEG = 1 << 30;
+// AG: checkpoint groups (128 columns) of a tile; BN: its dy columns; BT: tokens of
+// a block; RL, RC: blocks in flight as they lie in memory / widened; RA:
+// accumulators; CW, EW: converter and epilogue warps; SEG: token blocks that
+// accumulate in TMEM before the sums move to registers.
+//
+// Two groups share each load of dy: 50 KB of L2 traffic buy 256 x 256 x 64
+// products instead of 41 KB for half of them, which is what bounds one group
+// (65536 x (4096, 1024) bf16: 815 us).
+template <bool BF, int GROUPS>
+struct W8Half {
+    static constexpr bool BF16 = BF, F32 = false;
+    static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2, SEG = 1 << 30;
+    static constexpr int RL = AG == 1 ? 4 : 3, RC = AG == 1 ? 3 : 2, RA = AG == 1 ? 2 : 1;
+    static constexpr int CW = 8, EW = 8;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&t);
-    }
-};
-struct W8F16 {
-    static constexpr bool BF16 = false, F32 = false;
-    static constexpr int BN = 256, BT = 64, RL = 4, RC = 3, CW = 8, EW = 4, BYTES = 2;
-    static constexpr int SEG = 1 << 30;
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        const __half2 t = __floats2half2_rn(a, b);
-        return *reinterpret_cast<const uint32_t*>(&t);
+        if constexpr (BF) {
+            const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&t);
+        } else {
+            const __half2 t = __floats2half2_rn(a, b);
+            return *reinterpret_cast<const uint32_t*>(&t);
+        }
     }
 };
 // The tensor cores' fp32 accumulation truncates: its error grows with the number
@@ -90,19 +93,21 @@ struct W8F16 {
 // the result as near as an fp32 product's.
 struct W8F32 {
     static constexpr bool BF16 = true, F32 = true;
-    static constexpr int BN = 128, BT = 32, RL = 6, RC = 3, CW = 8, EW = 8, BYTES = 4;
-    static constexpr int SEG = 32;
+    static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4, SEG = 32;
+    static constexpr int RL = 6, RC = 3, RA = 2, CW = 8, EW = 8;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        return W8BF16::pack2(a, b);
+        return W8Half<true, 1>::pack2(a, b);
     }
 };
 template <class D>
 struct W8Smem {
     static constexpr int DY = D::BT * D::BN * D::BYTES;  // dy as it lies in memory
-    static constexpr int Q = D::BT * W8_BK;
-    static constexpr int FACT = 1024;                    // scale and row factor of BT tokens
+    static constexpr int Q1 = D::BT * W8_BK;              // one group's bytes
+    static constexpr int Q = D::AG * Q1;
+    static constexpr int FACT = 1024;                    // scales and row factor of BT tokens
     static constexpr int LOAD = DY + Q + FACT;
-    static constexpr int A = D::BT * W8_BK * 2;          // widened checkpoint
+    static constexpr int A1 = D::BT * W8_BK * 2;         // widened checkpoint, one group
+    static constexpr int A = D::AG * A1;
     static constexpr int DY3 = D::F32 ? 3 * D::BT * D::BN * 2 : 0;  // dy's bf16 parts
     static constexpr int CONV = A + DY3;
     static constexpr size_t BYTES = (size_t)D::RL * LOAD + (size_t)D::RC * CONV + 1024;
@@ -155,11 +160,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     w8_kernel(const W8Params p, const __grid_constant__ W8Maps maps) {
     using Sm = W8Smem<D>;
     constexpr int RL = D::RL, RC = D::RC, BN = D::BN, BT = D::BT;
-    constexpr int ACC = D::F32 ? 2 * BN : BN;  // TMEM columns of an accumulator
+    constexpr int AG = D::AG, RA = D::RA, KT = AG * W8_BK;
+    constexpr int ACC = D::F32 ? 2 * BN : AG * BN;  // TMEM columns of an accumulator
+    constexpr int ROW = AG * BT;                     // place of the row factors behind the scales
     constexpr int CT = 32 * D::CW;
     constexpr uint32_t IDESC = w8_idesc(BN, D::BF16);
     extern __shared__ float4 w8_smem4[];
-    __shared__ uint64_t full[RL], free_l[RL], conv[RC], free_c[RC], acc_full[2], acc_empty[2],
+    __shared__ uint64_t full[RL], free_l[RL], conv[RC], free_c[RC], acc_full[RA], acc_empty[RA],
         drained;
     __shared__ uint32_t tmem_base_s;
     __shared__ int abort_s;
@@ -168,13 +175,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         (reinterpret_cast<uintptr_t>(w8_smem4) + 1023) & ~(uintptr_t)1023);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-    const int64_t kt = (p.K + W8_BK - 1) / W8_BK, nt = (p.N + BN - 1) / BN;
+    const int64_t kt = (p.K + KT - 1) / KT, nt = (p.N + BN - 1) / BN;
     const int64_t tiles = kt * nt, units = tiles * p.slices;
     const int64_t nblk = (p.M + BT - 1) / BT;
     // unit u: slice, then tile with k fastest: CTAs that run together share tokens
     auto unit_of = [&](int64_t u, int64_t& k0, int64_t& n0, int64_t& b0, int& nb) {
         const int64_t z = u / tiles, t = u % tiles;
-        k0 = (t % kt) * W8_BK;
+        k0 = (t % kt) * KT;
         n0 = (t / kt) * BN;
         b0 = z * p.blocks;
         nb = (int)(min64(nblk, b0 + p.blocks) - b0);
@@ -197,14 +204,14 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             mbar_init(&conv[c], CT);
             mbar_init(&free_c[c], 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < RA; ++a) {
             mbar_init(&acc_full[a], 1);
             mbar_init(&acc_empty[a], 32 * D::EW);
         }
         mbar_init(&drained, 1);
         mbar_fence_init();
     }
-    if (warp == 1) tmem_alloc(&tmem_base_s, 2 * ACC);
+    if (warp == 1) tmem_alloc(&tmem_base_s, RA * ACC);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -219,7 +226,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            const int64_t g = k0 / W8_BK;
+            const int64_t g0 = k0 / W8_BK;
             for (int b = 0; b < nb; ++b, ++j, r.next()) {
                 const int s = r.s;
                 ok = __all_sync(0xffffffffu, ws_wait(&free_l[s], r.ph ^ 1u, abort, p.err));
@@ -235,13 +242,21 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                             tma_load_3d(slot_dy(s) + c * BT * 128, &maps.dy, (int)n0 + 64 * c,
                                         (int)m0, 0, &full[s]);
                     }
-                    tma_load_3d(slot_q(s), &maps.q, (int)k0, (int)m0, 0, &full[s]);
+#pragma unroll
+                    for (int g = 0; g < AG; ++g)
+                        tma_load_3d(slot_q(s) + g * Sm::Q1, &maps.q, (int)k0 + g * W8_BK, (int)m0, 0,
+                                    &full[s]);
                 }
                 for (int t = lane; t < BT; t += 32) {
                     const int64_t m = m0 + t;
                     const bool in = m < p.M;
-                    cp_async4(slot_f(s) + t, in ? p.scale + m * p.groups + g : p.scale, in);
-                    if (p.row) cp_async4(slot_f(s) + 128 + t, in ? p.row + m : p.row, in);
+#pragma unroll
+                    for (int g = 0; g < AG; ++g) {
+                        const bool have = in && g0 + g < p.groups;
+                        cp_async4(slot_f(s) + g * BT + t,
+                                  have ? p.scale + m * p.groups + g0 + g : p.scale, have);
+                    }
+                    if (p.row) cp_async4(slot_f(s) + ROW + t, in ? p.row + m : p.row, in);
                 }
                 cp_async_arrive(&full[s]);
             }
@@ -254,7 +269,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         if (lane == 0) {
             RingPos<RL> rl;
             RingPos<RC> rc;
-            RingPos<2> ra;
+            RingPos<RA> ra;
             bool ok = true;
             for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 int64_t k0, n0, b0;
@@ -275,13 +290,23 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     tc_fence_after();
                     const uint32_t sa = smem_u32(slot_a(c));
                     const uint32_t sb = smem_u32(D::F32 ? slot_dy3(c) : slot_dy(s));
+                    if constexpr (D::F32) {
 #pragma unroll
-                    for (int part = 0; part < (D::F32 ? 3 : 1); ++part)
+                        for (int part = 0; part < 3; ++part)
+#pragma unroll
+                            for (int kk = 0; kk < BT / 16; ++kk)
+                                umma_f16(acc + (part ? BN : 0), w8_desc<BT>(sa, kk),
+                                         w8_desc<BT>(sb + part * (BT * BN * 2), kk), IDESC,
+                                         (in_seg > 0 || part == 2 || kk > 0) ? 1u : 0u);
+                    } else {
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk)
-                            umma_f16(acc + (part ? BN : 0), w8_desc<BT>(sa, kk),
-                                     w8_desc<BT>(sb + part * (BT * BN * 2), kk), IDESC,
-                                     (in_seg > 0 || part == 2 || kk > 0) ? 1u : 0u);
+#pragma unroll
+                            for (int g = 0; g < AG; ++g)
+                                umma_f16(acc + g * BN, w8_desc<BT>(sa + g * Sm::A1, kk),
+                                         w8_desc<BT>(sb, kk), IDESC,
+                                         (in_seg > 0 || kk > 0) ? 1u : 0u);
+                    }
                     if constexpr (!D::F32) umma_commit(&free_l[s]);
                     umma_commit(&free_c[c]);
                     if (in_seg == D::SEG - 1 || b == nb - 1) {
@@ -314,10 +339,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 if (!ok) break;
                 const float* fs = slot_f(s);
 #pragma unroll
-                for (int i = 0; i < PIECES; ++i) {
+                for (int gi = 0; gi < AG * PIECES; ++gi) {
+                    const int g = gi / PIECES, i = gi % PIECES;
                     const int t = (ct >> 3) + i * (CT / 8);
-                    const uint4 w = *reinterpret_cast<const uint4*>(slot_q(s) + t * W8_BK + piece * 16);
-                    const float f = !D::F32 && p.row ? fs[t] * fs[128 + t] : fs[t];
+                    const uint4 w = *reinterpret_cast<const uint4*>(slot_q(s) + g * Sm::Q1 +
+                                                                    t * W8_BK + piece * 16);
+                    const float f =
+                        !D::F32 && p.row ? fs[g * BT + t] * fs[ROW + t] : fs[g * BT + t];
                     const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
                     uint32_t o[8];
 #pragma unroll
@@ -333,7 +361,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     // 8 neighbouring lanes then touch all 8 chunks of a row
                     const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
                     const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
-                    char* a = slot_a(cs);
+                    char* a = slot_a(cs) + g * Sm::A1;
                     *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + blk)) = blk ? hi : lo;
                     *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + 1 - blk)) = blk ? lo : hi;
                 }
@@ -349,7 +377,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                         const float4 a = swap ? x1 : x0, e = swap ? x0 : x1;
                         float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
                         if (p.row) {
-                            const float r = fs[128 + t];
+                            const float r = fs[ROW + t];
 #pragma unroll
                             for (int h = 0; h < 8; ++h) v[h] *= r;
                         }
@@ -379,20 +407,18 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         const int q = warp & 3;
         constexpr int COLS = BN / (D::EW / 4);
         const int col0 = ((warp - 2 - D::CW) >> 2) * COLS;
-        RingPos<2> ra;
+        RingPos<RA> ra;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            const int64_t k = k0 + q * 32 + lane;
-            const float cs = p.slices == 1 && p.col && k < p.K ? p.col[k] : 1.f;
             const int ncols = (int)min64(p.N - n0, BN);
-            float* pw = p.work ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k : nullptr;
-            const auto put = [&](int c, float v) {
+            const auto put = [&](int g, int c, float v) {
+                const int64_t k = k0 + g * W8_BK + q * 32 + lane;
                 if (c >= ncols || k >= p.K) return;
-                if (p.slices > 1) pw[(int64_t)c * p.ldp] = v;
-                else w8_store(p.dw, (n0 + c) * p.ldw + k, p.out_type, v * cs);
+                if (p.slices > 1) p.work[((u / tiles) * p.N + n0 + c) * p.ldp + k] = v;
+                else w8_store(p.dw, (n0 + c) * p.ldw + k, p.out_type, p.col ? v * p.col[k] : v);
             };
             if constexpr (D::F32) {
                 float sum[COLS];
@@ -419,7 +445,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 }
                 if (!ok) break;
 #pragma unroll
-                for (int i = 0; i < COLS; ++i) put(col0 + i, sum[i]);
+                for (int i = 0; i < COLS; ++i) put(0, col0 + i, sum[i]);
             } else {
                 const int a = ra.s;
                 ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
@@ -428,12 +454,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 tc_fence_after();
                 const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC);
 #pragma unroll 1
-                for (int c = 0; c < ncols; c += 32) {
+                for (int gc = 0; gc < AG * COLS; gc += 32) {
+                    const int g = gc / COLS, c = col0 + gc % COLS;
                     uint32_t r[32];
-                    tmem_ld32_issue(trow + (uint32_t)c, r);
+                    tmem_ld32_issue(trow + (uint32_t)(g * BN + c), r);
                     tmem_wait32(r);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) put(c + i, __uint_as_float(r[i]));
+                    for (int i = 0; i < 32; ++i) put(g, c + i, __uint_as_float(r[i]));
                     __syncwarp();
                 }
                 tc_fence_before();
@@ -445,7 +472,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     __syncthreads();
     if (warp == 1) {
         tc_fence_after();
-        tmem_dealloc(tmem, 2 * ACC);
+        tmem_dealloc(tmem, RA * ACC);
     }
 }
 
@@ -479,27 +506,29 @@ __global__ void __launch_bounds__(256)
 // more write and read of the result.
 struct W8Plan {
     int64_t slices, blocks;
+    double us;
 };
 template <class D>
 static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
-    const int64_t nblk = (M + D::BT - 1) / D::BT;
-    const int64_t tiles = (K + W8_BK - 1) / W8_BK * ((N + D::BN - 1) / D::BN);
-    const double block_us = D::F32 ? 0.22 : 0.30, tile_us = 2.0;
+    const int64_t nblk = (M + D::BT - 1) / D::BT, kt = D::AG * W8_BK;
+    const int64_t tiles = (K + kt - 1) / kt * ((N + D::BN - 1) / D::BN);
+    const double block_us = D::F32 ? 0.25 : D::AG == 1 ? 0.45 : 0.60;
+    const double tile_us = 1.0 + D::AG * (D::F32 ? 0.5 : 1.0);
     const double slice_us = 2.0 * (double)N * (double)K * 4.0 / 5e6;
-    W8Plan best{1, nblk};
-    double least = 1e30;
+    W8Plan best{1, nblk, 1e30};
     for (int64_t s = 1; s <= nblk && s <= 148; ++s) {
         const int64_t per = (nblk + s - 1) / s;
         if ((nblk + per - 1) / per != s) continue;  // the same as a smaller count
         const int64_t rounds = (tiles * s + 147) / 148;
         const double t = (double)rounds * ((double)per * block_us + tile_us) +
                          (s > 1 ? 2.0 + (double)s * slice_us : 0.0);
-        if (t < least) {
-            least = t;
-            best = {s, per};
-        }
+        if (t < best.us) best = {s, per, t};
     }
     return best;
+}
+// 16-bit dy: one group a tile or two, whichever is estimated faster
+static bool w8_two_groups(int64_t M, int64_t N, int64_t K) {
+    return w8_plan<W8Half<true, 2>>(M, N, K).us < w8_plan<W8Half<true, 1>>(M, N, K).us;
 }
 static int64_t w8_pitch(int64_t K) { return (K + 3) / 4 * 4; }
 
@@ -520,7 +549,8 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     static int attr[MMB_MAX_DEVICES] = {};
     const int st = mmb_smem_attr(w8_kernel<D>, W8Smem<D>::BYTES, attr);
     if (st != MMB_OK) return st;
-    const int64_t units = (p.K + W8_BK - 1) / W8_BK * ((p.N + D::BN - 1) / D::BN) * p.slices;
+    const int64_t kt = D::AG * W8_BK;
+    const int64_t units = (p.K + kt - 1) / kt * ((p.N + D::BN - 1) / D::BN) * p.slices;
     w8_kernel<D><<<(unsigned)min64(units, 148), w8_threads<D>(), W8Smem<D>::BYTES, s>>>(p, maps);
     const int rc = mmb_launch_status();
     if (rc != MMB_OK || p.slices == 1) return rc;
@@ -536,7 +566,9 @@ using namespace mmb;
 
 extern "C" size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int32_t dy_type) {
     if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
-    const W8Plan plan = dy_type == MMB_F32 ? w8_plan<W8F32>(M, N, K) : w8_plan<W8BF16>(M, N, K);
+    const W8Plan plan = dy_type == MMB_F32        ? w8_plan<W8F32>(M, N, K)
+                        : w8_two_groups(M, N, K) ? w8_plan<W8Half<true, 2>>(M, N, K)
+                                                 : w8_plan<W8Half<true, 1>>(M, N, K);
     return plan.slices > 1 ? (size_t)plan.slices * (size_t)N * (size_t)w8_pitch(K) : 0;
 }
 
@@ -571,6 +603,10 @@ extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, c
     p.dw = dw; p.ldw = ldw; p.out_type = out_type; p.work = work;
     p.err = mmb_device_error_flag();
     if (dy_type == MMB_F32) return w8_launch<W8F32>(p, dy, lddy, q, ldq, s);
-    if (dy_type == MMB_BF16) return w8_launch<W8BF16>(p, dy, lddy, q, ldq, s);
-    return w8_launch<W8F16>(p, dy, lddy, q, ldq, s);
+    const bool two = w8_two_groups(M, N, K);
+    if (dy_type == MMB_BF16)
+        return two ? w8_launch<W8Half<true, 2>>(p, dy, lddy, q, ldq, s)
+                   : w8_launch<W8Half<true, 1>>(p, dy, lddy, q, ldq, s);
+    return two ? w8_launch<W8Half<false, 2>>(p, dy, lddy, q, ldq, s)
+               : w8_launch<W8Half<false, 1>>(p, dy, lddy, q, ldq, s);
 }
