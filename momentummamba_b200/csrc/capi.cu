@@ -124,13 +124,13 @@ static mmb_encode_tiled_fn encode_fn() {
 
 bool mmb_encode_tile_map(CUtensorMap* map, const void* base, int elem_bytes, int64_t dim0,
                          int64_t dim1, int64_t dim2, int64_t stride1, int64_t stride2,
-                         int box0, int box1, int swizzle_bytes) {
+                         int box0, int box1, int swizzle_bytes, int box2) {
     mmb_encode_tiled_fn fn = encode_fn();
     if (!fn) return false;
     const cuuint64_t dims[3] = {(cuuint64_t)dim0, (cuuint64_t)dim1, (cuuint64_t)dim2};
     const cuuint64_t strides[2] = {(cuuint64_t)(stride1 * elem_bytes),
                                    (cuuint64_t)(stride2 * elem_bytes)};
-    const cuuint32_t box[3] = {(cuuint32_t)box0, (cuuint32_t)box1, 1};
+    const cuuint32_t box[3] = {(cuuint32_t)box0, (cuuint32_t)box1, (cuuint32_t)box2};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUtensorMapSwizzle sw = swizzle_bytes == MMB_SWZ_128B_ATOM32
                                       ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B

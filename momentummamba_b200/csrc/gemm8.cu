@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(G8_NT, 1)
         }
         for (int a = 0; a < 2; ++a) {
             mbar_init(&acc_full[a], 1);
-            mbar_init(&acc_empty[a], 32 * G8_EW);
+            mbar_init(&acc_empty[a], G8_EW);
         }
         mbar_init(&drained, 1);
         mbar_fence_init();
@@ -322,7 +322,7 @@ __global__ void __launch_bounds__(G8_NT, 1)
                 if (c + 32 < PER) tmem_wait32(r[cur ^ 1]);
             }
             tc_fence_before();
-            mbar_arrive(&acc_empty[ra.s]);
+            warp_arrive(&acc_empty[ra.s]);
         }
         if (lane == 0) bulk_wait_read<0>();
         __syncwarp();

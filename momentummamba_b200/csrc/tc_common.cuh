@@ -115,11 +115,30 @@ __device__ __forceinline__ void bulk_wait_read() {
 }
 
 // Bounded wait on phase `parity` that also gives up when another role aborted.
+// A poll may suspend the thread for up to WS_HINT_NS: waiting warps that poll
+// without one take most of the SM's issue slots from those that work (a third of
+// all instructions in the weight-gradient kernel were polls).  WS_POLLS of them
+// take about two seconds.
+constexpr uint32_t WS_HINT_NS = 20000;
+constexpr int WS_POLLS = 100000;
+__device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(WS_HINT_NS)
+        : "memory");
+    return ok != 0;
+}
 __device__ __forceinline__ bool ws_wait(uint64_t* bar, uint32_t parity, volatile int* abort,
                                         int* err) {
-    for (int i = 0; i < MMB_WAIT_POLLS; ++i) {
-        if (mbar_try_wait(bar, parity)) return true;
+    if (mbar_try_wait_hint(bar, parity)) return true;
+#pragma unroll 1
+    for (int i = 0; i < WS_POLLS; ++i) {
         if (*abort) return false;
+        if (mbar_try_wait_hint(bar, parity)) return true;
     }
     *abort = 1;
     if (err) atomicOr(err, 1);
@@ -127,6 +146,32 @@ __device__ __forceinline__ bool ws_wait(uint64_t* bar, uint32_t parity, volatile
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+// 16 bytes of shared memory by their 32-bit address (a generic pointer's accesses
+// go the longer way of global ones)
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ float lds4f(uint32_t a) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, const uint4& v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z),
+                 "r"(v.w)
+                 : "memory");
+}
+
+// One arrival for a whole warp: 256 threads that arrive one by one keep the barrier
+// busy for about 1000 cycles.
+__device__ __forceinline__ void warp_arrive(uint64_t* bar) {
+    __syncwarp();
+    if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
 // Barrier `ID` over THREADS threads of the CTA: true on all of them when `ok` was.

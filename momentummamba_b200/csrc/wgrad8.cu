@@ -113,7 +113,7 @@ struct W8Smem {
     static constexpr size_t BYTES = (size_t)D::RL * LOAD + (size_t)D::RC * CONV + 1024;
 };
 template <class D>
-__host__ __device__ constexpr int w8_threads() { return 32 * (2 + D::CW + D::EW); }
+__host__ __device__ constexpr int w8_threads() { return 32 * (3 + D::CW + D::EW); }
 
 // `bar` counts an arrival of this lane once its cp.async copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
@@ -134,6 +134,7 @@ struct W8Params {
     int out_type;
     float* work;  // more slices: (slices, N, ldp) partial sums
     int64_t ldp;
+    int dy_blocks, q_blocks;  // tensor maps by column blocks: one box a tile (see w8_launch)
     int* err;
 };
 struct W8Maps {
@@ -146,13 +147,23 @@ __device__ __forceinline__ void w8_store(void* dw, int64_t at, int out_type, flo
     else static_cast<__half*>(dw)[at] = __float2half_rn(v);
 }
 
-// 4 bytes -> 4 floats: a byte with its sign bit flipped becomes the low mantissa
-// bits of 2^23, from which 2^23 + 128 is taken away
-__device__ __forceinline__ void w8_widen4(uint32_t w, float2& v0, float2& v1) {
+// 4 bytes q -> 4 floats q * f.  A byte with its sign bit flipped, q + 128, becomes
+// the second byte of the mantissa of 2^15; one fused step then takes 2^15 + 128
+// away and multiplies: (2^15 + 128 + q) * f - (2^15 + 128) * f.  With f held to 15
+// significant bits (w8_factor) both products' difference is exact.
+__device__ __forceinline__ void w8_widen4(uint32_t w, float f, float fc, float2& v0, float2& v1) {
     const uint32_t u = w ^ 0x80808080u;
-    const auto at = [&](int j) { return __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 + j)); };
-    v0 = fadd2(make_float2(at(0), at(1)), f2(-8388736.f));
-    v1 = fadd2(make_float2(at(2), at(3)), f2(-8388736.f));
+    v0 = ffma2(make_float2(__uint_as_float(__byte_perm(u, 0x47000000u, 0x7404)),
+                           __uint_as_float(__byte_perm(u, 0x47000000u, 0x7414))), f2(f), f2(fc));
+    v1 = ffma2(make_float2(__uint_as_float(__byte_perm(u, 0x47000000u, 0x7424)),
+                           __uint_as_float(__byte_perm(u, 0x47000000u, 0x7434))), f2(f), f2(fc));
+}
+constexpr float W8_HUGE = 0x1p111f;
+// f rounded to 15 significant bits: exact for a power of two; with a row factor
+// 2^-16 of the value, far below the rounding to 16 bits that follows.
+__device__ __forceinline__ float w8_factor(float f) {
+    const uint32_t u = __float_as_uint(f);
+    return (u & 0x7f800000u) == 0x7f800000u ? f : __uint_as_float((u + 0x100u) & ~0x1ffu);
 }
 
 template <class D>
@@ -198,15 +209,15 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         abort_s = 0;
         for (int s = 0; s < RL; ++s) {
             mbar_init(&full[s], 1 + 32);               // TMA, and the factors of each lane
-            mbar_init(&free_l[s], D::F32 ? CT : 1);    // read by the converters / by the MMAs
+            mbar_init(&free_l[s], D::F32 ? D::CW : 1);  // read by the converters / by the MMAs
         }
         for (int c = 0; c < RC; ++c) {
-            mbar_init(&conv[c], CT);
+            mbar_init(&conv[c], D::CW);
             mbar_init(&free_c[c], 1);
         }
         for (int a = 0; a < RA; ++a) {
             mbar_init(&acc_full[a], 1);
-            mbar_init(&acc_empty[a], 32 * D::EW);
+            mbar_init(&acc_empty[a], D::EW);
         }
         mbar_init(&drained, 1);
         mbar_fence_init();
@@ -218,52 +229,75 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     const uint32_t tmem = tmem_base_s;
 
     if (warp == 0) {
-        // ---- producer: tiles by TMA (lane 0), the tokens' factors by cp.async ----
+        // ---- producer ----
+        if (lane == 0) {
+            RingPos<RL> r;
+            int64_t j = 0;
+            bool ok = true;
+            for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
+                int64_t k0, n0, b0;
+                int nb;
+                unit_of(u, k0, n0, b0, nb);
+                const int kx = (int)k0, nx = (int)n0, kg = (int)(k0 / W8_BK), ng = (int)(n0 / 64);
+                int m0 = (int)(b0 * BT);
+                for (int b = 0; b < nb; ++b, ++j, m0 += BT, r.next()) {
+                    uint64_t* bar = &full[r.s];
+                    ok = ws_wait(&free_l[r.s], r.ph ^ 1u, abort, p.err);
+                    if (!ok) break;
+                    mbar_expect_tx(bar, Sm::DY + Sm::Q);
+                    if constexpr (D::F32) {
+                        tma_load_3d(slot_dy(r.s), &maps.dy, nx, m0, 0, bar);
+                    } else if (p.dy_blocks) {
+                        tma_load_3d(slot_dy(r.s), &maps.dy, 0, m0, ng, bar);
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < BN / 64; ++c)
+                            tma_load_3d(slot_dy(r.s) + c * BT * 128, &maps.dy, nx + 64 * c, m0, 0, bar);
+                    }
+                    if (AG == 1 || p.q_blocks) {
+                        tma_load_3d(slot_q(r.s), &maps.q, AG == 1 ? kx : 0, m0, AG == 1 ? 0 : kg, bar);
+                    } else {
+#pragma unroll
+                        for (int g = 0; g < AG; ++g)
+                            tma_load_3d(slot_q(r.s) + g * Sm::Q1, &maps.q, kx + g * W8_BK, m0, 0, bar);
+                    }
+                }
+            }
+            // copies still in flight land before the CTA leaves
+            for (int64_t q = j - RL > 0 ? j - RL : 0; q < j; ++q)
+                mbar_wait_polls(&full[q % RL], (uint32_t)((q / RL) & 1), 1 << 16);
+        }
+    } else if (warp == 2) {
+        // ---- the tokens' factors, a token or two a lane, by cp.async ----
         RingPos<RL> r;
-        int64_t j = 0;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
             const int64_t g0 = k0 / W8_BK;
-            for (int b = 0; b < nb; ++b, ++j, r.next()) {
-                const int s = r.s;
-                ok = __all_sync(0xffffffffu, ws_wait(&free_l[s], r.ph ^ 1u, abort, p.err));
+            int64_t m = b0 * BT + lane;
+            const float* sc = p.scale + m * p.groups + g0;
+            const int64_t next = 32 * p.groups;
+            for (int b = 0; b < nb; ++b, r.next()) {
+                ok = __all_sync(0xffffffffu, ws_wait(&free_l[r.s], r.ph ^ 1u, abort, p.err));
                 if (!ok) break;
-                const int64_t m0 = (b0 + b) * BT;
-                if (lane == 0) {
-                    mbar_expect_tx(&full[s], Sm::DY + Sm::Q);
-                    if constexpr (D::F32) {
-                        tma_load_3d(slot_dy(s), &maps.dy, (int)n0, (int)m0, 0, &full[s]);
-                    } else {
+                float* f = slot_f(r.s) + lane;
 #pragma unroll
-                        for (int c = 0; c < BN / 64; ++c)
-                            tma_load_3d(slot_dy(s) + c * BT * 128, &maps.dy, (int)n0 + 64 * c,
-                                        (int)m0, 0, &full[s]);
-                    }
-#pragma unroll
-                    for (int g = 0; g < AG; ++g)
-                        tma_load_3d(slot_q(s) + g * Sm::Q1, &maps.q, (int)k0 + g * W8_BK, (int)m0, 0,
-                                    &full[s]);
-                }
-                for (int t = lane; t < BT; t += 32) {
-                    const int64_t m = m0 + t;
+                for (int t = 0; t < BT; t += 32, m += 32, sc += next) {
                     const bool in = m < p.M;
 #pragma unroll
                     for (int g = 0; g < AG; ++g) {
-                        const bool have = in && g0 + g < p.groups;
-                        cp_async4(slot_f(s) + g * BT + t,
-                                  have ? p.scale + m * p.groups + g0 + g : p.scale, have);
+                        const bool have = in && (AG == 1 || g0 + g < p.groups);
+                        cp_async4(f + g * BT + t, have ? sc + g : p.scale, have);
                     }
-                    if (p.row) cp_async4(slot_f(s) + ROW + t, in ? p.row + m : p.row, in);
+                    if (p.row) cp_async4(f + ROW + t, in ? p.row + m : p.row, in);
                 }
-                cp_async_arrive(&full[s]);
+                cp_async_arrive(&full[r.s]);
             }
         }
-        // copies still in flight land before the CTA leaves
-        for (int64_t q = j - RL > 0 ? j - RL : 0; q < j; ++q)
-            mbar_wait_polls(&full[q % RL], (uint32_t)((q / RL) & 1), 1 << 16);
+        cp_async_commit();
+        cp_async_wait<0>();
     } else if (warp == 1) {
         // ---- MMA issuer ----
         if (lane == 0) {
@@ -319,10 +353,10 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             umma_commit(&drained);
             mbar_wait_polls(&drained, 0, 1 << 20);
         }
-    } else if (warp < 2 + D::CW) {
+    } else if (warp < 3 + D::CW) {
         // ---- converters ----
         constexpr int PIECES = BT * W8_BK / 16 / CT;  // 16-byte pieces of q a thread and block
-        const int ct = tid - 64;
+        const int ct = tid - 96;
         const int piece = ct & 7;  // the piece's 16 columns; token ct / 8 + i * CT / 8
         const int blk = piece >> 2, c0 = (piece & 3) * 2;
         RingPos<RL> rl;
@@ -337,51 +371,70 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 ok = ws_wait(&free_c[cs], rc.ph ^ 1u, abort, p.err) &&
                      ws_wait(&full[s], rl.ph, abort, p.err);
                 if (!ok) break;
-                const float* fs = slot_f(s);
+                const uint32_t fs = smem_u32(slot_f(s)), qs = smem_u32(slot_q(s)) + piece * 16;
+                const uint32_t as = smem_u32(slot_a(cs));
+                // every load before the first store, which would hold later loads back
+                uint4 w[AG * PIECES];
+                float fa[AG * PIECES];
+                bool huge = false;
 #pragma unroll
                 for (int gi = 0; gi < AG * PIECES; ++gi) {
-                    const int g = gi / PIECES, i = gi % PIECES;
-                    const int t = (ct >> 3) + i * (CT / 8);
-                    const uint4 w = *reinterpret_cast<const uint4*>(slot_q(s) + g * Sm::Q1 +
-                                                                    t * W8_BK + piece * 16);
-                    const float f =
-                        !D::F32 && p.row ? fs[g * BT + t] * fs[ROW + t] : fs[g * BT + t];
-                    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-                    uint32_t o[8];
-#pragma unroll
-                    for (int h = 0; h < 4; ++h) {
-                        float2 v0, v1;
-                        w8_widen4(ws[h], v0, v1);
-                        v0 = fmul2(v0, f2(f));
-                        v1 = fmul2(v1, f2(f));
-                        o[2 * h] = D::pack2(v0.x, v0.y);
-                        o[2 * h + 1] = D::pack2(v1.x, v1.y);
-                    }
-                    // the two column blocks write their chunks in opposite order:
-                    // 8 neighbouring lanes then touch all 8 chunks of a row
-                    const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
-                    const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
-                    char* a = slot_a(cs) + g * Sm::A1;
-                    *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + blk)) = blk ? hi : lo;
-                    *reinterpret_cast<uint4*>(a + w8_chunk<BT>(blk, t, c0 + 1 - blk)) = blk ? lo : hi;
+                    const int g = gi / PIECES, t = (ct >> 3) + gi % PIECES * (CT / 8);
+                    w[gi] = lds16(qs + g * Sm::Q1 + t * W8_BK);
+                    fa[gi] = lds4f(fs + 4 * (g * BT + t));
+                    if (!D::F32 && p.row) fa[gi] *= lds4f(fs + 4 * (ROW + t));
+                    huge |= fabsf(fa[gi]) >= W8_HUGE;
                 }
+                const auto widen = [&](float shrink, float grow) {
+#pragma unroll
+                    for (int gi = 0; gi < AG * PIECES; ++gi) {
+                        const int g = gi / PIECES, t = (ct >> 3) + gi % PIECES * (CT / 8);
+                        const float f = w8_factor(fa[gi] * shrink), fc = -32896.f * f;
+                        const uint32_t ws[4] = {w[gi].x, w[gi].y, w[gi].z, w[gi].w};
+                        uint32_t o[8];
+#pragma unroll
+                        for (int h = 0; h < 4; ++h) {
+                            float2 v0, v1;
+                            w8_widen4(ws[h], f, fc, v0, v1);
+                            o[2 * h] = D::pack2(v0.x * grow, v0.y * grow);
+                            o[2 * h + 1] = D::pack2(v1.x * grow, v1.y * grow);
+                        }
+                        // the two column blocks write their chunks in opposite order:
+                        // 8 neighbouring lanes then touch all 8 chunks of a row
+                        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
+                        const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
+                        const uint32_t a = as + g * Sm::A1;
+                        sts16(a + w8_chunk<BT>(blk, t, c0 + blk), blk ? hi : lo);
+                        sts16(a + w8_chunk<BT>(blk, t, c0 + 1 - blk), blk ? lo : hi);
+                    }
+                };
+                // factors of 2^111 and more (values near the type's own limit) go in two
+                // steps: 2^15 times them would be an infinity
+                if (__any_sync(0xffffffffu, huge)) widen(0x1p-32f, 0x1p32f);
+                else widen(1.f, 1.f);
                 if constexpr (D::F32) {
                     // dy * row = high + middle + low, each bf16: 8 values a step
                     const int c = ct & 15, swap = (ct >> 2) & 1;
+                    constexpr int STEPS = BT * BN / 8 / CT;
+                    const uint32_t ds = smem_u32(slot_dy(s)) + c * 32;
+                    uint4 x[STEPS][2];
+                    float r[STEPS];
 #pragma unroll
-                    for (int i = 0; i < BT * BN / 8 / CT; ++i) {
+                    for (int i = 0; i < STEPS; ++i) {
                         const int t = (ct >> 4) + i * (CT / 16);
-                        const float4* src =
-                            reinterpret_cast<const float4*>(slot_dy(s) + t * (BN * 4) + c * 32);
-                        const float4 x0 = src[swap], x1 = src[swap ^ 1];
-                        const float4 a = swap ? x1 : x0, e = swap ? x0 : x1;
-                        float v[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
-                        if (p.row) {
-                            const float r = fs[ROW + t];
+                        x[i][0] = lds16(ds + t * (BN * 4) + 16 * swap);
+                        x[i][1] = lds16(ds + t * (BN * 4) + 16 * (swap ^ 1));
+                        r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
+                    }
 #pragma unroll
-                            for (int h = 0; h < 8; ++h) v[h] *= r;
-                        }
-                        char* dst = slot_dy3(cs) + w8_chunk<BT>(c >> 3, t, c & 7);
+                    for (int i = 0; i < STEPS; ++i) {
+                        const int t = (ct >> 4) + i * (CT / 16);
+                        const uint4 a = swap ? x[i][1] : x[i][0], e = swap ? x[i][0] : x[i][1];
+                        const uint32_t raw[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
+                        float v[8];
+#pragma unroll
+                        for (int h = 0; h < 8; ++h) v[h] = __uint_as_float(raw[h]) * r[i];
+                        const uint32_t dst = as + Sm::A + w8_chunk<BT>(c >> 3, t, c & 7);
 #pragma unroll
                         for (int part = 0; part < 3; ++part) {
                             uint32_t o[4];
@@ -391,14 +444,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                                 v[2 * h] -= bf16_lo(o[h]);
                                 v[2 * h + 1] -= bf16_hi(o[h]);
                             }
-                            *reinterpret_cast<uint4*>(dst + part * (BT * BN * 2)) =
-                                make_uint4(o[0], o[1], o[2], o[3]);
+                            sts16(dst + part * (BT * BN * 2), make_uint4(o[0], o[1], o[2], o[3]));
                         }
                     }
                 }
                 fence_proxy_async_smem();
-                mbar_arrive(&conv[cs]);
-                if constexpr (D::F32) mbar_arrive(&free_l[s]);
+                warp_arrive(&conv[cs]);
+                if constexpr (D::F32) warp_arrive(&free_l[s]);
             }
         }
     } else {
@@ -406,7 +458,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         // every 4 warps a share of the columns n ----
         const int q = warp & 3;
         constexpr int COLS = BN / (D::EW / 4);
-        const int col0 = ((warp - 2 - D::CW) >> 2) * COLS;
+        const int col0 = ((warp - 3 - D::CW) >> 2) * COLS;
         RingPos<RA> ra;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
@@ -441,7 +493,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                             for (int i = 0; i < 16; ++i) sum[c + i] += r[i];
                         }
                     tc_fence_before();
-                    mbar_arrive(&acc_empty[a]);
+                    warp_arrive(&acc_empty[a]);
                 }
                 if (!ok) break;
 #pragma unroll
@@ -464,7 +516,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     __syncwarp();
                 }
                 tc_fence_before();
-                mbar_arrive(&acc_empty[a]);
+                warp_arrive(&acc_empty[a]);
             }
         }
     }
@@ -541,11 +593,22 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     p.ldp = w8_pitch(p.K);
     if (p.slices > 1 && !p.work) return MMB_ERR_WORKSPACE;
     W8Maps maps;
+    // 16-bit dy and a pair of groups as (column in a block, token, block) where their
+    // widths are whole blocks: one copy a tile instead of one a block (a copy costs the
+    // producer about 200 cycles)
+    p.dy_blocks = !D::F32 && p.N % 64 == 0;
+    p.q_blocks = D::AG > 1 && p.K % W8_BK == 0;
     const bool okd =
         D::F32 ? mmb_encode_tile_map(&maps.dy, dy, 4, p.N, p.M, 1, lddy, lddy * p.M, D::BN, D::BT, 0)
-               : mmb_encode_tile_map(&maps.dy, dy, 2, p.N, p.M, 1, lddy, lddy * p.M, 64, D::BT, 128);
-    if (!okd || !mmb_encode_tile_map(&maps.q, q, 1, p.K, p.M, 1, ldq, ldq * p.M, W8_BK, D::BT, 0))
-        return MMB_ERR_ALIGN;
+        : p.dy_blocks
+            ? mmb_encode_tile_map(&maps.dy, dy, 2, 64, p.M, p.N / 64, lddy, 64, 64, D::BT, 128,
+                                  D::BN / 64)
+            : mmb_encode_tile_map(&maps.dy, dy, 2, p.N, p.M, 1, lddy, lddy * p.M, 64, D::BT, 128);
+    const bool okq = p.q_blocks ? mmb_encode_tile_map(&maps.q, q, 1, W8_BK, p.M, p.K / W8_BK, ldq,
+                                                      W8_BK, W8_BK, D::BT, 0, D::AG)
+                                : mmb_encode_tile_map(&maps.q, q, 1, p.K, p.M, 1, ldq, ldq * p.M,
+                                                      W8_BK, D::BT, 0);
+    if (!okd || !okq) return MMB_ERR_ALIGN;
     static int attr[MMB_MAX_DEVICES] = {};
     const int st = mmb_smem_attr(w8_kernel<D>, W8Smem<D>::BYTES, attr);
     if (st != MMB_OK) return st;

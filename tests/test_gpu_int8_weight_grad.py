@@ -158,3 +158,17 @@ def test_refusals():
            None, 0, dw.data_ptr(), 128, None, None)
     assert lib.mmb_wgrad_ck8_work_floats(40000, 128, 128, 0) > 0
     assert lib.mmb_wgrad_ck8(*big) == 5         # several slices and no workspace: refused before any launch
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_values_at_the_types_own_limit(dtype):
+    """Rows at the lowest value beside ordinary ones: finite products stay finite and exact."""
+    from momentummamba_b200 import int8
+    M, N, K = 130, 24, 160
+    x, dy, _, _ = make(M, N, K, dtype)
+    x[17] = torch.finfo(dtype).min
+    x[40, 130:] = 1e36
+    dy[17] = 0
+    dy[40] *= 1e-30
+    ck = int8.checkpoint_rows(x)
+    check(int8.weight_grad_ckpt(dy, ck), dy, ck.restore(), None, None, dtype)
