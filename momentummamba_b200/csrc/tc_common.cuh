@@ -167,6 +167,10 @@ __device__ __forceinline__ void sts16(uint32_t a, const uint4& v) {
                  : "memory");
 }
 
+__device__ __forceinline__ void sts8(uint32_t a, uint32_t x, uint32_t y) {
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
+}
+
 // One arrival for a whole warp: 256 threads that arrive one by one keep the barrier
 // busy for about 1000 cycles.
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {

@@ -41,23 +41,25 @@ __host__ __device__ constexpr uint32_t w8_idesc(int n, bool bf16) {
     return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | (1u << 15) |
            (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
-__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc,
+// alo, blo: the low words of the operands' descriptors; they share the high one
+__device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t alo, uint32_t blo, uint32_t dhi,
                                          uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d_tmem),
+        "r"(alo), "r"(blo), "r"(dhi), "r"(idesc), "r"(accumulate)
         : "memory");
 }
 
 // Operand layout of BT tokens: blocks of 64 columns, each BT rows (tokens) of
 // 128 bytes with the 128-byte swizzle: 16-byte chunk c of token t lies at chunk
-// c ^ (t % 8).  Step kk is 16 tokens on.
-template <int BT>
-__device__ __forceinline__ uint64_t w8_desc(uint32_t saddr, int kk) {
-    return smem_desc(saddr + kk * 16 * 128, BT * 128, 1024, W8_SWZ128);
-}
+// c ^ (t % 8).  An MMA's step is 16 tokens on.
+// In a descriptor's low word, 16 bytes count 1: the issuing thread adds offsets to
+// words made once (made anew for each MMA they took it 100 cycles apiece).
+constexpr uint32_t W8_STEP = 16 * 128 / 16;
 template <int BT>
 __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
     return (uint32_t)(block * (BT * 128) + t * 128 + ((c ^ (t & 7)) << 4));
@@ -203,7 +205,6 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         return reinterpret_cast<float*>(smem + s * Sm::LOAD + Sm::DY + Sm::Q);
     };
     auto slot_a = [&](int c) { return smem + RL * Sm::LOAD + c * Sm::CONV; };
-    auto slot_dy3 = [&](int c) { return smem + RL * Sm::LOAD + c * Sm::CONV + Sm::A; };
 
     if (tid == 0) {
         abort_s = 0;
@@ -305,6 +306,8 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             RingPos<RC> rc;
             RingPos<RA> ra;
             bool ok = true;
+            const uint64_t d0 = smem_desc(smem_u32(smem), BT * 128, 1024, W8_SWZ128);
+            const uint32_t lo0 = (uint32_t)d0, dhi = (uint32_t)(d0 >> 32);
             for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
                 int64_t k0, n0, b0;
                 int nb;
@@ -322,24 +325,24 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     ok = ws_wait(&conv[c], rc.ph, abort, p.err);
                     if (!ok) break;
                     tc_fence_after();
-                    const uint32_t sa = smem_u32(slot_a(c));
-                    const uint32_t sb = smem_u32(D::F32 ? slot_dy3(c) : slot_dy(s));
+                    const uint32_t la = lo0 + (RL * Sm::LOAD + c * Sm::CONV) / 16;
+                    const uint32_t lb = D::F32 ? la + Sm::A / 16 : lo0 + s * (Sm::LOAD / 16);
+                    const uint32_t first = in_seg > 0 ? 1u : 0u;
                     if constexpr (D::F32) {
 #pragma unroll
                         for (int part = 0; part < 3; ++part)
 #pragma unroll
                             for (int kk = 0; kk < BT / 16; ++kk)
-                                umma_f16(acc + (part ? BN : 0), w8_desc<BT>(sa, kk),
-                                         w8_desc<BT>(sb + part * (BT * BN * 2), kk), IDESC,
-                                         (in_seg > 0 || part == 2 || kk > 0) ? 1u : 0u);
+                                umma_f16(acc + (part ? BN : 0), la + kk * W8_STEP,
+                                         lb + part * (BT * BN * 2 / 16) + kk * W8_STEP, dhi, IDESC,
+                                         part == 2 || kk > 0 ? 1u : first);
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk)
 #pragma unroll
                             for (int g = 0; g < AG; ++g)
-                                umma_f16(acc + g * BN, w8_desc<BT>(sa + g * Sm::A1, kk),
-                                         w8_desc<BT>(sb, kk), IDESC,
-                                         (in_seg > 0 || kk > 0) ? 1u : 0u);
+                                umma_f16(acc + g * BN, la + g * (Sm::A1 / 16) + kk * W8_STEP,
+                                         lb + kk * W8_STEP, dhi, IDESC, kk > 0 ? 1u : first);
                     }
                     if constexpr (!D::F32) umma_commit(&free_l[s]);
                     umma_commit(&free_c[c]);
@@ -357,8 +360,11 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         // ---- converters ----
         constexpr int PIECES = BT * W8_BK / 16 / CT;  // 16-byte pieces of q a thread and block
         const int ct = tid - 96;
-        const int piece = ct & 7;  // the piece's 16 columns; token ct / 8 + i * CT / 8
-        const int blk = piece >> 2, c0 = (piece & 3) * 2;
+        // a piece is 16 columns of a token; 8 neighbouring lanes take the first block's
+        // pieces of one token and the second's of its neighbour, so that their stores
+        // touch all 8 chunks of a row
+        const int piece = ct & 7, blk = piece >> 2, c0 = (piece & 3) * 2;
+        const int t0 = 2 * (ct >> 4) + (((ct >> 3) & 1) ^ blk);
         RingPos<RL> rl;
         RingPos<RC> rc;
         bool ok = true;
@@ -379,7 +385,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 bool huge = false;
 #pragma unroll
                 for (int gi = 0; gi < AG * PIECES; ++gi) {
-                    const int g = gi / PIECES, t = (ct >> 3) + gi % PIECES * (CT / 8);
+                    const int g = gi / PIECES, t = t0 + gi % PIECES * (CT / 8);
                     w[gi] = lds16(qs + g * Sm::Q1 + t * W8_BK);
                     fa[gi] = lds4f(fs + 4 * (g * BT + t));
                     if (!D::F32 && p.row) fa[gi] *= lds4f(fs + 4 * (ROW + t));
@@ -388,7 +394,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 const auto widen = [&](float shrink, float grow) {
 #pragma unroll
                     for (int gi = 0; gi < AG * PIECES; ++gi) {
-                        const int g = gi / PIECES, t = (ct >> 3) + gi % PIECES * (CT / 8);
+                        const int g = gi / PIECES, t = t0 + gi % PIECES * (CT / 8);
                         const float f = w8_factor(fa[gi] * shrink), fc = -32896.f * f;
                         const uint32_t ws[4] = {w[gi].x, w[gi].y, w[gi].z, w[gi].w};
                         uint32_t o[8];
@@ -399,13 +405,9 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                             o[2 * h] = D::pack2(v0.x * grow, v0.y * grow);
                             o[2 * h + 1] = D::pack2(v1.x * grow, v1.y * grow);
                         }
-                        // the two column blocks write their chunks in opposite order:
-                        // 8 neighbouring lanes then touch all 8 chunks of a row
-                        const uint4 lo = make_uint4(o[0], o[1], o[2], o[3]);
-                        const uint4 hi = make_uint4(o[4], o[5], o[6], o[7]);
                         const uint32_t a = as + g * Sm::A1;
-                        sts16(a + w8_chunk<BT>(blk, t, c0 + blk), blk ? hi : lo);
-                        sts16(a + w8_chunk<BT>(blk, t, c0 + 1 - blk), blk ? lo : hi);
+                        sts16(a + w8_chunk<BT>(blk, t, c0), make_uint4(o[0], o[1], o[2], o[3]));
+                        sts16(a + w8_chunk<BT>(blk, t, c0 + 1), make_uint4(o[4], o[5], o[6], o[7]));
                     }
                 };
                 // factors of 2^111 and more (values near the type's own limit) go in two
@@ -413,38 +415,42 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 if (__any_sync(0xffffffffu, huge)) widen(0x1p-32f, 0x1p32f);
                 else widen(1.f, 1.f);
                 if constexpr (D::F32) {
-                    // dy * row = high + middle + low, each bf16: 8 values a step
-                    const int c = ct & 15, swap = (ct >> 2) & 1;
+                    // dy * row = high + middle + low, each bf16: 4 columns of either
+                    // block of 64 a step (16 lanes then cover a row of each)
+                    const int c = ct & 15;
                     constexpr int STEPS = BT * BN / 8 / CT;
-                    const uint32_t ds = smem_u32(slot_dy(s)) + c * 32;
+                    const uint32_t ds = smem_u32(slot_dy(s)) + c * 16;
                     uint4 x[STEPS][2];
                     float r[STEPS];
 #pragma unroll
                     for (int i = 0; i < STEPS; ++i) {
                         const int t = (ct >> 4) + i * (CT / 16);
-                        x[i][0] = lds16(ds + t * (BN * 4) + 16 * swap);
-                        x[i][1] = lds16(ds + t * (BN * 4) + 16 * (swap ^ 1));
+                        x[i][0] = lds16(ds + t * (BN * 4));
+                        x[i][1] = lds16(ds + t * (BN * 4) + 256);
                         r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
                     }
 #pragma unroll
                     for (int i = 0; i < STEPS; ++i) {
                         const int t = (ct >> 4) + i * (CT / 16);
-                        const uint4 a = swap ? x[i][1] : x[i][0], e = swap ? x[i][0] : x[i][1];
-                        const uint32_t raw[8] = {a.x, a.y, a.z, a.w, e.x, e.y, e.z, e.w};
-                        float v[8];
 #pragma unroll
-                        for (int h = 0; h < 8; ++h) v[h] = __uint_as_float(raw[h]) * r[i];
-                        const uint32_t dst = as + Sm::A + w8_chunk<BT>(c >> 3, t, c & 7);
+                        for (int h = 0; h < 2; ++h) {
+                            const uint32_t dst =
+                                as + Sm::A + w8_chunk<BT>(h, t, c >> 1) + (c & 1) * 8;
+                            float2 v0 = make_float2(__uint_as_float(x[i][h].x),
+                                                    __uint_as_float(x[i][h].y));
+                            float2 v1 = make_float2(__uint_as_float(x[i][h].z),
+                                                    __uint_as_float(x[i][h].w));
+                            v0 = fmul2(v0, f2(r[i]));
+                            v1 = fmul2(v1, f2(r[i]));
 #pragma unroll
-                        for (int part = 0; part < 3; ++part) {
-                            uint32_t o[4];
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                o[h] = D::pack2(v[2 * h], v[2 * h + 1]);
-                                v[2 * h] -= bf16_lo(o[h]);
-                                v[2 * h + 1] -= bf16_hi(o[h]);
+                            for (int part = 0; part < 3; ++part) {
+                                const uint32_t o0 = D::pack2(v0.x, v0.y), o1 = D::pack2(v1.x, v1.y);
+                                sts8(dst + part * (BT * BN * 2), o0, o1);
+                                v0.x -= bf16_lo(o0);
+                                v0.y -= bf16_hi(o0);
+                                v1.x -= bf16_lo(o1);
+                                v1.y -= bf16_hi(o1);
                             }
-                            sts16(dst + part * (BT * BN * 2), make_uint4(o[0], o[1], o[2], o[3]));
                         }
                     }
                 }
