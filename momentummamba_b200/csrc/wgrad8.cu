@@ -16,7 +16,8 @@
 //     q * s * row is rounded to that type, half a unit of 2^-8 (bf16) or 2^-11
 //     (fp16), below the half step that q itself is off by.
 //   * fp32 dy (times row, in fp32) is split into three bf16 parts, 24 bits in
-//     all, and multiplied with the exact q * s in three MMAs.
+//     all, and multiplied with the exact q * s: the high part into one
+//     accumulator, the two small ones into another.
 //
 // Tile: one or two groups of 128 checkpoint columns (a token has one scale in
 // each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a token's
@@ -67,7 +68,8 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 
 // AG: checkpoint groups (128 columns) of a tile; BN: its dy columns; BT: tokens of
 // a block; RL, RC: blocks in flight as they lie in memory / widened; RA:
-// accumulators; CW, EW: converter and epilogue warps; SEG: token blocks that
+// accumulators; CW, EW: converter (in CG groups, each at a block of its own) and
+// epilogue warps; SEG: token blocks that
 // accumulate in TMEM before the sums move to registers.
 //
 // Two groups share each load of dy: 50 KB of L2 traffic buy 256 x 256 x 64
@@ -78,7 +80,7 @@ struct W8Half {
     static constexpr bool BF16 = BF, F32 = false;
     static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2, SEG = 1 << 30;
     static constexpr int RL = AG == 1 ? 4 : 3, RC = AG == 1 ? 3 : 2, RA = AG == 1 ? 2 : 1;
-    static constexpr int CW = 8, EW = 8;
+    static constexpr int CW = 8, CG = 1, EW = 8;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         if constexpr (BF) {
             const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
@@ -96,7 +98,7 @@ struct W8Half {
 struct W8F32 {
     static constexpr bool BF16 = true, F32 = true;
     static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4, SEG = 32;
-    static constexpr int RL = 6, RC = 3, RA = 2, CW = 8, EW = 8;
+    static constexpr int RL = 4, RC = 4, RA = 2, CW = 8, CG = 4, EW = 8;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return W8Half<true, 1>::pack2(a, b);
     }
@@ -176,7 +178,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     constexpr int AG = D::AG, RA = D::RA, KT = AG * W8_BK;
     constexpr int ACC = D::F32 ? 2 * BN : AG * BN;  // TMEM columns of an accumulator
     constexpr int ROW = AG * BT;                     // place of the row factors behind the scales
-    constexpr int CT = 32 * D::CW;
+    constexpr int CGW = D::CW / D::CG, CT = 32 * CGW;  // a converter group
     constexpr uint32_t IDESC = w8_idesc(BN, D::BF16);
     extern __shared__ float4 w8_smem4[];
     __shared__ uint64_t full[RL], free_l[RL], conv[RC], free_c[RC], acc_full[RA], acc_empty[RA],
@@ -210,10 +212,10 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         abort_s = 0;
         for (int s = 0; s < RL; ++s) {
             mbar_init(&full[s], 1 + 32);               // TMA, and the factors of each lane
-            mbar_init(&free_l[s], D::F32 ? D::CW : 1);  // read by the converters / by the MMAs
+            mbar_init(&free_l[s], D::F32 ? CGW : 1);  // read by the converters / by the MMAs
         }
         for (int c = 0; c < RC; ++c) {
-            mbar_init(&conv[c], D::CW);
+            mbar_init(&conv[c], CGW);
             mbar_init(&free_c[c], 1);
         }
         for (int a = 0; a < RA; ++a) {
@@ -329,13 +331,15 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     const uint32_t lb = D::F32 ? la + Sm::A / 16 : lo0 + s * (Sm::LOAD / 16);
                     const uint32_t first = in_seg > 0 ? 1u : 0u;
                     if constexpr (D::F32) {
+                        // high and middle parts lie side by side: one MMA of twice the
+                        // columns reads the checkpoint once for both
 #pragma unroll
-                        for (int part = 0; part < 3; ++part)
-#pragma unroll
-                            for (int kk = 0; kk < BT / 16; ++kk)
-                                umma_f16(acc + (part ? BN : 0), la + kk * W8_STEP,
-                                         lb + part * (BT * BN * 2 / 16) + kk * W8_STEP, dhi, IDESC,
-                                         part == 2 || kk > 0 ? 1u : first);
+                        for (int kk = 0; kk < BT / 16; ++kk) {
+                            umma_f16(acc, la + kk * W8_STEP, lb + kk * W8_STEP, dhi,
+                                     w8_idesc(2 * BN, true), kk > 0 ? 1u : first);
+                            umma_f16(acc + BN, la + kk * W8_STEP,
+                                     lb + 2 * (BT * BN * 2 / 16) + kk * W8_STEP, dhi, IDESC, 1u);
+                        }
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk)
@@ -359,7 +363,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     } else if (warp < 3 + D::CW) {
         // ---- converters ----
         constexpr int PIECES = BT * W8_BK / 16 / CT;  // 16-byte pieces of q a thread and block
-        const int ct = tid - 96;
+        const int group = (warp - 3) / CGW, ct = (tid - 96) % CT;
         // a piece is 16 columns of a token; 8 neighbouring lanes take the first block's
         // pieces of one token and the second's of its neighbour, so that their stores
         // touch all 8 chunks of a row
@@ -367,12 +371,14 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         const int t0 = 2 * (ct >> 4) + (((ct >> 3) & 1) ^ blk);
         RingPos<RL> rl;
         RingPos<RC> rc;
+        RingPos<D::CG> turn;
         bool ok = true;
         for (int64_t u = blockIdx.x; u < units && ok; u += gridDim.x) {
             int64_t k0, n0, b0;
             int nb;
             unit_of(u, k0, n0, b0, nb);
-            for (int b = 0; b < nb; ++b, rl.next(), rc.next()) {
+            for (int b = 0; b < nb; ++b, rl.next(), rc.next(), turn.next()) {
+                if (turn.s != group) continue;
                 const int s = rl.s, cs = rc.s;
                 ok = ws_wait(&free_c[cs], rc.ph ^ 1u, abort, p.err) &&
                      ws_wait(&full[s], rl.ph, abort, p.err);
@@ -472,11 +478,24 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             int nb;
             unit_of(u, k0, n0, b0, nb);
             const int ncols = (int)min64(p.N - n0, BN);
-            const auto put = [&](int g, int c, float v) {
-                const int64_t k = k0 + g * W8_BK + q * 32 + lane;
-                if (c >= ncols || k >= p.K) return;
-                if (p.slices > 1) p.work[((u / tiles) * p.N + n0 + c) * p.ldp + k] = v;
-                else w8_store(p.dw, (n0 + c) * p.ldw + k, p.out_type, p.col ? v * p.col[k] : v);
+            float* slice = p.slices > 1 ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k0 : nullptr;
+            // V columns n0 + c .. of this lane's column k
+            const auto put = [&](int g, int c, const auto& v) {
+                constexpr int V = sizeof(v) / sizeof(v[0]);
+                const int kr = g * W8_BK + q * 32 + lane;
+                if (k0 + kr >= p.K) return;
+                if (slice) {
+                    float* w = slice + c * p.ldp + kr;
+#pragma unroll
+                    for (int i = 0; i < V; ++i, w += p.ldp)
+                        if (c + i < ncols) *w = v[i];
+                } else {
+                    const float cs = p.col ? p.col[k0 + kr] : 1.f;
+                    int64_t at = (n0 + c) * p.ldw + k0 + kr;
+#pragma unroll
+                    for (int i = 0; i < V; ++i, at += p.ldw)
+                        if (c + i < ncols) w8_store(p.dw, at, p.out_type, v[i] * cs);
+                }
             };
             if constexpr (D::F32) {
                 float sum[COLS];
@@ -502,8 +521,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     warp_arrive(&acc_empty[a]);
                 }
                 if (!ok) break;
-#pragma unroll
-                for (int i = 0; i < COLS; ++i) put(0, col0 + i, sum[i]);
+                put(0, col0, sum);
             } else {
                 const int a = ra.s;
                 ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
@@ -514,11 +532,9 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 #pragma unroll 1
                 for (int gc = 0; gc < AG * COLS; gc += 32) {
                     const int g = gc / COLS, c = col0 + gc % COLS;
-                    uint32_t r[32];
-                    tmem_ld32_issue(trow + (uint32_t)(g * BN + c), r);
-                    tmem_wait32(r);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) put(g, c + i, __uint_as_float(r[i]));
+                    float v[32];
+                    tmem_ld32(trow + (uint32_t)(g * BN + c), v);
+                    put(g, c, v);
                     __syncwarp();
                 }
                 tc_fence_before();
