@@ -311,11 +311,24 @@ __global__ void __launch_bounds__(G8_NT, 1)
                                 bulk_commit();
                             }
                         }
-                    } else if (m < p.M) {
-                        T* o = static_cast<T*>(p.out) + m * p.ldo + nt0 + col;
+                    } else {
+                        // rows of any alignment: through the box, then a token at a time
+                        // with a column a lane (a token a lane took 32 sectors a store)
+                        uint4* row = reinterpret_cast<uint4*>(box + lane * 128);
+                        __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + j < ncols) o[j] = O::from_f(v[j]);
+                        for (int j = 0; j < 8; ++j)
+                            row[j ^ (lane & 7)] = make_uint4(
+                                __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                                __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+                        __syncwarp();
+                        const int rows = (int)min64(p.M - (m - lane), 32);
+                        T* o = static_cast<T*>(p.out) + (m - lane) * p.ldo + nt0 + col + lane;
+                        const float* b = reinterpret_cast<const float*>(box);
+                        if (col + lane < ncols)
+#pragma unroll 8
+                            for (int t = 0; t < rows; ++t, o += p.ldo)
+                                *o = O::from_f(b[t * 32 + (((lane >> 2) ^ (t & 7)) << 2) + (lane & 3)]);
                     }
                 }
                 __syncwarp();

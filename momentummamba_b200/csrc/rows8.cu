@@ -227,23 +227,24 @@ __device__ __forceinline__ float r8_max(float a, float b) {
     return d;
 }
 
-// Sum and maximum over the row: the warp's lanes, then the row's warps (whose
-// number is the block's x extent / 32; blocks of several warps hold one row).
+// Sum (and maximum) over the row: LPR lanes, then the row's warps (whose number is
+// the block's x extent / 32; blocks of several warps hold one row).
+template <int LPR, bool MAX>
 __device__ __forceinline__ void r8_row_reduce(float& sum, float& top, float2* part) {
 #pragma unroll
-    for (int m = 16; m >= 1; m >>= 1) {
+    for (int m = LPR / 2; m >= 1; m >>= 1) {
         sum += __shfl_xor_sync(0xffffffffu, sum, m);
-        top = r8_max(top, __shfl_xor_sync(0xffffffffu, top, m));
+        if constexpr (MAX) top = r8_max(top, __shfl_xor_sync(0xffffffffu, top, m));
     }
     const int nw = blockDim.x >> 5;
-    if (nw == 1) return;
+    if (LPR < 32 || nw == 1) return;
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(sum, top);
     __syncthreads();
     sum = 0.f;
     top = 0.f;
     for (int w = 0; w < nw; ++w) {
         sum += part[w].x;
-        top = r8_max(top, part[w].y);
+        if constexpr (MAX) top = r8_max(top, part[w].y);
     }
 }
 
@@ -268,12 +269,17 @@ struct R8Fwd {
 };
 
 // CK: checkpoint form (groups, powers of two); else 8-bit rows.
-template <class EX, class ER, bool VEC, int NC, int NT, bool CK>
+// LPR: lanes of a row, 16 for rows of at most 128 columns (two rows a warp).
+template <class EX, class ER, bool VEC, int NC, int NT, bool CK, int LPR = 32>
 __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
     __shared__ float2 part[R8_MAX_WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
-    if (row >= p.rows) return;  // whole warps; blocks of several warps hold one row
+    constexpr int RPW = 32 / LPR;
+    const int lane = threadIdx.x & (LPR - 1), warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int64_t first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * RPW;
+    if (first >= p.rows) return;  // whole warps; blocks of several warps hold one row
+    // a half warp past the end goes through the last row again and stores nothing
+    const int64_t at = first + (threadIdx.x & 31) / LPR, row = min64(at, p.rows - 1);
+    const int64_t cols = at < p.rows ? p.cols : 0;  // columns that are stored
     const auto col0 = [&](int c) { return (int64_t)(c * nw + warp) * R8_CHUNK; };
     const auto* xr = static_cast<const typename EX::T*>(p.x) + row * p.xs;
 
@@ -303,7 +309,7 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
     if (p.h) {
         auto* hr = static_cast<typename ER::T*>(p.h) + row * p.hs;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) r8_store<ER, VEC>(hr, col0(c), lane, p.cols, v[c]);
+        for (int c = 0; c < NC; ++c) r8_store<ER, VEC>(hr, col0(c), lane, cols, v[c]);
     }
     float sum = 0.f, top = 0.f;
     if (p.norm) {
@@ -329,7 +335,7 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) top = r8_max(top, fabsf(v[c][j]));
     }
-    if (p.norm || !CK) r8_row_reduce(sum, top, part);
+    if (p.norm || !CK) r8_row_reduce<LPR, !CK>(sum, top, part);
     const float rstd = p.norm ? __frsqrt_rn(__fdiv_rn(sum, (float)p.cols) + p.eps) : 1.f;
     int8_t* qr = p.q ? p.q + row * p.qs : nullptr;
 
@@ -341,11 +347,11 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
             uint32_t b[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) b[j] = r8_round(__fmul_rn(v[c][j], inv));
-            r8_store_q<VEC>(qr, col0(c), lane, p.cols, b);
+            r8_store_q<VEC>(qr, col0(c), lane, cols, b);
         }
         // rounded down: 127 scales never exceed the row's largest value, which may
         // be the type's own
-        if (lane == 0 && warp == 0)
+        if (lane == 0 && warp == 0 && cols)
             p.scale[row] = top < INFINITY ? __fdiv_rd(top * rstd, 127.f) : NAN;
         return;
     } else {
@@ -394,14 +400,14 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
                     for (int j = 0; j < V; ++j) b[V * g + j] = r8_round(q[j]);
                     const int64_t gc = col0(c) + (VEC ? (lane >> 4) : g) * R8_GROUP;
                     const bool mine = VEC ? (lane & 15) == 0 : lane == 0;
-                    if (mine && gc < p.cols)
+                    if (mine && gc < cols)
                         sr[gc / R8_GROUP] =
                             t[g] < INFINITY ? __uint_as_float((uint32_t)(127 + e) << 23) : NAN;
                 }
-                r8_store_q<VEC>(qr, col0(c), lane, p.cols, b);
+                r8_store_q<VEC>(qr, col0(c), lane, cols, b);
             }
         }
-        if (p.rstd && lane == 0 && warp == 0) p.rstd[row] = rstd;
+        if (p.rstd && lane == 0 && warp == 0 && cols) p.rstd[row] = rstd;
         if (p.n) {
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -418,13 +424,13 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
                 }
                 if (p.nt == MMB_F32)
                     r8_store<T8F32, VEC>(static_cast<float*>(p.n) + row * p.ns, col0(c), lane,
-                                         p.cols, o);
+                                         cols, o);
                 else if (p.nt == MMB_BF16)
                     r8_store<T8BF16, VEC>(static_cast<__nv_bfloat16*>(p.n) + row * p.ns, col0(c),
-                                          lane, p.cols, o);
+                                          lane, cols, o);
                 else
                     r8_store<T8F16, VEC>(static_cast<__half*>(p.n) + row * p.ns, col0(c), lane,
-                                         p.cols, o);
+                                         cols, o);
             }
         }
     }
@@ -452,14 +458,16 @@ struct R8Bwd {
 // registers; at the end a block's rows-in-flight are added up in shared memory
 // and the block writes its own line of partial sums, which r8_colsum_kernel adds
 // in a fixed order: the result does not depend on timing.
-template <class EN, class EX, bool VEC, int NC, int U, int NT>
+template <class EN, class EX, bool VEC, int NC, int U, int NT, int LPR = 32>
 __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
     extern __shared__ float r8_acc[];  // blockDim.y x cols, when blockDim.y > 1
     __shared__ float2 part[R8_MAX_WARPS];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    constexpr int RPW = 32 / LPR;
+    const int lane = threadIdx.x & (LPR - 1), warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const int sub = (threadIdx.x & 31) / LPR;  // this half warp's row
     const int64_t groups = (p.cols + R8_GROUP - 1) / R8_GROUP;
     const auto col0 = [&](int c) { return (int64_t)(c * nw + warp) * R8_CHUNK; };
-    const int64_t step = (int64_t)gridDim.x * blockDim.y;
+    const int64_t step = (int64_t)gridDim.x * blockDim.y * RPW;
     constexpr int G = VEC ? 1 : 2;  // groups a lane's 8 values fall into
     float acc[NC][8];
 #pragma unroll
@@ -467,7 +475,7 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[c][j] = 0.f;
 
-    for (int64_t row0 = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row0 < p.rows;
+    for (int64_t row0 = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * RPW; row0 < p.rows;
          row0 += step * U) {
         R8Load<EN, VEC> ln[U][NC];
         R8Load<EX, VEC> lh[U][NC];
@@ -476,7 +484,7 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             // a row past the end loads the last one again and stores nothing
-            const int64_t row = min64(row0 + u * step, p.rows - 1);
+            const int64_t row = min64(row0 + sub + u * step, p.rows - 1);
             const auto* dnr = static_cast<const typename EN::T*>(p.dn) + row * p.dns;
 #pragma unroll
             for (int c = 0; c < NC; ++c) ln[u][c].load(dnr, col0(c), lane, p.cols);
@@ -498,8 +506,9 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
         }
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int64_t row = row0 + u * step;
-            if (row >= p.rows) break;  // the same for a whole warp, and for a block of one row
+            if (row0 + u * step >= p.rows) break;  // the same for a warp, and for a block of one row
+            const int64_t row = row0 + sub + u * step;
+            const bool live = RPW == 1 || row < p.rows;
             float z[NC][8], g[NC][8], dot = 0.f;
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
@@ -508,7 +517,7 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     z[c][j] *= s[u][c][VEC ? 0 : j >> 2] * rstd[u];
-                    acc[c][j] = fmaf(g[c][j], z[c][j], acc[c][j]);
+                    if (live) acc[c][j] = fmaf(g[c][j], z[c][j], acc[c][j]);
                 }
                 if (p.w) {
                     R8Load<T8F32, VEC> lw;
@@ -522,7 +531,7 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
                 for (int j = 0; j < 8; ++j) dot = fmaf(g[c][j], z[c][j], dot);
             }
             float unused = 0.f;
-            r8_row_reduce(dot, unused, part);
+            r8_row_reduce<LPR, false>(dot, unused, part);
             const float mean = __fdiv_rn(dot, (float)p.cols);
             auto* dxr = static_cast<typename EX::T*>(p.dx) + row * p.dxs;
 #pragma unroll
@@ -535,12 +544,16 @@ __global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) g[c][j] += a[j];
                 }
-                r8_store<EX, VEC>(dxr, col0(c), lane, p.cols, g[c]);
+                if (live) r8_store<EX, VEC>(dxr, col0(c), lane, p.cols, g[c]);
             }
             if (nw > 1) __syncthreads();  // `part` is written again for the next row
         }
     }
     if (!p.part) return;
+    if constexpr (RPW == 2) {  // the half warps' rows; both then write the same sums
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[0][j] += __shfl_xor_sync(0xffffffffu, acc[0][j], 16);
+    }
     float* out = p.part + (int64_t)blockIdx.x * p.cols;
     if (blockDim.y == 1) {
 #pragma unroll
@@ -631,10 +644,12 @@ __global__ void __launch_bounds__(256)
 // ---------------------------------------------------------------------------
 // Warps per row, chunks per warp and rows per block.  NC = 0: too wide.
 struct R8Shape {
-    int warps, nc, rows;
+    int warps, nc, rows;  // rows: of a block
+    bool half;            // two rows a warp
 };
-static R8Shape r8_shape(int64_t cols) {
+static R8Shape r8_shape(int64_t cols, bool vec) {
     const int64_t chunks = (cols + R8_CHUNK - 1) / R8_CHUNK;
+    if (vec && cols <= 128) return {1, 1, 8, true};
     if (chunks <= 1) return {1, 1, 4};
     if (chunks <= 2) return {1, 2, 4};
     if (chunks <= 4) return {1, 4, 4};
@@ -656,8 +671,13 @@ static bool r8_aligned_q(const void* p, int64_t stride) {
 
 template <class EX, class ER, bool VEC, bool CK>
 static int r8_fwd_launch(const R8Fwd& p, const R8Shape& s, cudaStream_t st) {
-    const dim3 block(32 * s.warps, s.rows);
+    const dim3 block(32 * s.warps, s.half ? s.rows / 2 : s.rows);
     const unsigned grid = (unsigned)((p.rows + s.rows - 1) / s.rows);
+    if constexpr (VEC)
+        if (s.half) {
+            r8_fwd_kernel<EX, ER, true, 1, 128, CK, 16><<<grid, block, 0, st>>>(p);
+            return mmb_launch_status();
+        }
     if (s.nc == 1) r8_fwd_kernel<EX, ER, VEC, 1, 128, CK><<<grid, block, 0, st>>>(p);
     else if (s.nc == 2 && s.warps == 1)
         r8_fwd_kernel<EX, ER, VEC, 2, 128, CK><<<grid, block, 0, st>>>(p);
@@ -674,12 +694,12 @@ static int r8_fwd_form(const R8Fwd& p, const R8Shape& s, bool vec, bool ck, cuda
               : r8_fwd_launch<EX, ER, false, false>(p, s, st);
 }
 static int r8_fwd(const R8Fwd& p, int xt, int rt, bool ck, cudaStream_t st) {
-    const R8Shape s = r8_shape(p.cols);
-    if (!s.nc) return MMB_ERR_UNSUPPORTED;
     const int xb = r8_bytes(xt), rb = r8_bytes(rt);
     const bool vec = p.cols % 8 == 0 && r8_aligned(p.x, p.xs, xb) && r8_aligned(p.res, p.rs, rb) &&
                      r8_aligned(p.h, p.hs, rb) && r8_aligned(p.n, p.ns, r8_bytes(p.nt)) &&
                      r8_aligned(p.w, 0, 4) && r8_aligned_q(p.q, p.qs);
+    const R8Shape s = r8_shape(p.cols, vec);
+    if (!s.nc) return MMB_ERR_UNSUPPORTED;
     if (xt == MMB_F32) return r8_fwd_form<T8F32, T8F32>(p, s, vec, ck, st);
     if (xt == MMB_BF16)
         return rt == MMB_F32 ? r8_fwd_form<T8BF16, T8F32>(p, s, vec, ck, st)
@@ -703,13 +723,18 @@ static int r8_fwd_check(const R8Fwd& p, int xt, int rt) {
 // partial sums stay small.
 static int r8_bwd_blocks(int64_t rows, const R8Shape& s) {
     const int64_t need = (rows + s.rows - 1) / s.rows;
-    const int64_t most = 148 * (s.warps * s.rows <= 4 ? 4 : s.warps <= 8 ? 2 : 1);
+    const int64_t most = 148 * (s.warps == 1 ? 4 : s.warps <= 8 ? 2 : 1);
     return (int)min64(need, most);
 }
 template <class EN, class EX, bool VEC>
 static int r8_bwd_launch(const R8Bwd& p, const R8Shape& s, int blocks, cudaStream_t st) {
-    const dim3 block(32 * s.warps, s.rows);
-    const size_t sm = s.rows > 1 ? (size_t)s.rows * p.cols * sizeof(float) : 0;  // <= 16 KB
+    const dim3 block(32 * s.warps, s.half ? s.rows / 2 : s.rows);
+    const size_t sm = s.rows > 1 ? (size_t)block.y * p.cols * sizeof(float) : 0;  // <= 16 KB
+    if constexpr (VEC)
+        if (s.half) {
+            r8_bwd_kernel<EN, EX, true, 1, 2, 128, 16><<<blocks, block, sm, st>>>(p);
+            return mmb_launch_status();
+        }
     if (s.nc == 1) r8_bwd_kernel<EN, EX, VEC, 1, 4, 128><<<blocks, block, sm, st>>>(p);
     else if (s.nc == 2 && s.warps == 1)
         r8_bwd_kernel<EN, EX, VEC, 2, 2, 128><<<blocks, block, sm, st>>>(p);
@@ -757,8 +782,11 @@ extern "C" int mmb_norm_ck8_fwd(int64_t rows, int64_t cols, int32_t x_type, cons
 
 extern "C" size_t mmb_norm_ck8_bwd_work_floats(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    const R8Shape s = r8_shape(cols);
-    return s.nc ? (size_t)r8_bwd_blocks(rows, s) * (size_t)cols : 0;
+    // the loads' form is not known here: the larger of the two
+    const R8Shape a = r8_shape(cols, false), b = r8_shape(cols, true);
+    if (!a.nc) return 0;
+    const int na = r8_bwd_blocks(rows, a), nb = r8_bwd_blocks(rows, b);
+    return (size_t)(na > nb ? na : nb) * (size_t)cols;
 }
 
 extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, const void* dn,
@@ -778,8 +806,6 @@ extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, con
     if (!dn || !q || !scale || !rstd || !dx) return MMB_ERR_NULL;
     if (dweight && !work) return MMB_ERR_WORKSPACE;
     if (lddn < cols || (dh && lddh < cols) || ldq < cols || lddx < cols) return MMB_ERR_SHAPE;
-    const R8Shape s = r8_shape(cols);
-    if (!s.nc) return MMB_ERR_UNSUPPORTED;
     R8Bwd p{};
     p.rows = rows; p.cols = cols; p.dn = dn; p.dns = lddn; p.dh = dh; p.dhs = lddh; p.w = weight;
     p.q = q; p.qs = ldq; p.scale = scale; p.rstd = rstd; p.dx = dx; p.dxs = lddx;
@@ -787,6 +813,8 @@ extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, con
     const int nb = r8_bytes(dn_type), xb = r8_bytes(dx_type);
     const bool vec = cols % 8 == 0 && r8_aligned(dn, lddn, nb) && r8_aligned(dh, lddh, xb) &&
                      r8_aligned(dx, lddx, xb) && r8_aligned(weight, 0, 4) && r8_aligned_q(q, ldq);
+    const R8Shape s = r8_shape(cols, vec);
+    if (!s.nc) return MMB_ERR_UNSUPPORTED;
     const int blocks = r8_bwd_blocks(rows, s);
     int rc;
 #define R8_BWD(EN, EX)                                                \

@@ -87,6 +87,21 @@ def _ld(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
+def _lines(t: torch.Tensor, cols: int):
+    """(t as rows that the kernels take, their stride)."""
+    if t.is_contiguous():
+        return t, cols
+    t = _rows2(t)
+    return t, _ld(t)
+
+
+def _like(t: torch.Tensor, dtype: torch.dtype) -> torch.Tensor:
+    """A new contiguous tensor of t's shape."""
+    if dtype == t.dtype and t.is_contiguous():
+        return torch.empty_like(t, requires_grad=False)
+    return torch.empty(t.shape, dtype=dtype, device=t.device)
+
+
 def _weight(weight: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]:
     if weight is None:
         return None
@@ -97,9 +112,14 @@ def _weight(weight: Optional[torch.Tensor], cols: int) -> Optional[torch.Tensor]
     return weight
 
 
+_entry = {}
+
+
 def _call(name: str, idx: int, *args) -> None:
     """One library call on the current stream of device idx."""
-    fn = getattr(_lib.load(), name)
+    fn = _entry.get(name)
+    if fn is None:
+        fn = _entry[name] = getattr(_lib.load(), name)
     if idx == _get_device():
         st = fn(*args, _raw_stream(idx))
     else:
@@ -182,11 +202,12 @@ def _restore(q, scale, grouped, dtype):
     idx = _index(q, scale)
     code = _out_type(dtype)
     out = torch.empty(q.shape, dtype=dtype, device=q.device)
-    q2 = _rows2(q)
-    rows, cols = q2.shape
-    if rows and cols:
+    n = out.numel()
+    if n:
+        cols = q.shape[-1]
+        q2, ldq = _lines(q, cols)
         scale = scale.contiguous()
-        _call("mmb_restore_q8", idx, rows, cols, q2.data_ptr(), _ld(q2), scale.data_ptr(), grouped,
+        _call("mmb_restore_q8", idx, n // cols, cols, q2.data_ptr(), ldq, scale.data_ptr(), grouped,
               code, out.data_ptr(), cols)
     return out
 
@@ -196,20 +217,21 @@ def _norm_q8(x, weight, residual, eps, norm, what):
     xt = rt = _type(x, what + ": x")
     cols = _check_rows(x, residual, what)
     weight = _weight(weight, cols)
-    x2, dev = _rows2(x), x.device
-    rows = x2.shape[0]
+    x2, ldx = _lines(x, cols)
+    rows, dev = x.numel() // cols, x.device
     h = rp = hp = None
     ldr = cols
     if residual is not None:
         rt = _TYPES[residual.dtype]
-        r2 = _rows2(residual)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        rp, hp, ldr = r2.data_ptr(), h.data_ptr(), _ld(r2)
+        r2, ldr = _lines(residual, cols)
+        h = _like(residual, residual.dtype)
+        rp, hp = r2.data_ptr(), h.data_ptr()
     q = _empty_q(rows, cols, dev)
-    scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=dev)
+    scale = torch.empty(*x.shape[:-1], dtype=torch.float32, device=dev) if x.dim() > 1 else \
+        torch.empty((), dtype=torch.float32, device=dev)
     if rows:
-        _call("mmb_norm_q8", idx, rows, cols, xt, x2.data_ptr(), _ld(x2), rt, rp, ldr, _p(weight),
-              eps, norm, hp, cols, q.data_ptr(), _ld(q), scale.data_ptr())
+        _call("mmb_norm_q8", idx, rows, cols, xt, x2.data_ptr(), ldx, rt, rp, ldr, _p(weight),
+              eps, norm, hp, cols, q.data_ptr(), q.stride(0), scale.data_ptr())
     if x.dim() != 2:
         q = q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0]
     return Q8Rows(q, scale), h
@@ -287,29 +309,29 @@ def _norm_ckpt(x, weight, residual, eps, norm, n_dtype, keep, what):
     xt = rt = _type(x, what + ": x")
     cols = _check_rows(x, residual, what)
     weight = _weight(weight, cols)
-    x2, dev = _rows2(x), x.device
-    rows = x2.shape[0]
-    h = n = q = stats = rp = hp = sp = vp = None
-    ldr = cols
+    x2, ldx = _lines(x, cols)
+    rows, dev = x.numel() // cols, x.device
+    h = n = q = stats = rp = hp = np_ = qp = sp = vp = None
+    ldr = ldq = cols
     if residual is not None:
         rt = _TYPES[residual.dtype]
-        r2 = _rows2(residual)
-        h = torch.empty(x.shape, dtype=residual.dtype, device=dev)
-        rp, hp, ldr = r2.data_ptr(), h.data_ptr(), _ld(r2)
+        r2, ldr = _lines(residual, cols)
+        h = _like(residual, residual.dtype)
+        rp, hp = r2.data_ptr(), h.data_ptr()
     nt = 0
     if n_dtype is not None:
         nt = _out_type(n_dtype)
-        n = torch.empty(x.shape, dtype=n_dtype, device=dev)
+        n = _like(x, n_dtype)
+        np_ = n.data_ptr()
     if keep:
         groups = -(-cols // GROUP)
         q = _empty_q(rows, cols, dev)
         stats = torch.empty(rows * (groups + norm), dtype=torch.float32, device=dev)
-        sp = stats.data_ptr()
+        qp, ldq, sp = q.data_ptr(), q.stride(0), stats.data_ptr()
         vp = sp + 4 * rows * groups if norm else None
     if rows:
-        _call("mmb_norm_ck8_fwd", idx, rows, cols, xt, x2.data_ptr(), _ld(x2), rt, rp, ldr,
-              _p(weight), eps, norm, hp, cols, nt, _p(n), cols, _p(q),
-              cols if q is None else _ld(q), sp, vp)
+        _call("mmb_norm_ck8_fwd", idx, rows, cols, xt, x2.data_ptr(), ldx, rt, rp, ldr, _p(weight),
+              eps, norm, hp, cols, nt, np_, cols, qp, ldq, sp, vp)
     return n, h, q, stats
 
 
@@ -329,7 +351,7 @@ def _wgrad_floats(M: int, N: int, K: int, code: int) -> int:
     return _lib.load().mmb_wgrad_ck8_work_floats(M, N, K, code)
 
 
-def _norm_ckpt_bwd(dn, dh, weight, q, stats, shape, out_dtype, want_dw):
+def _norm_ckpt_bwd(dn, dh, weight, q, stats, out_dtype, want_dw):
     """(dx, dweight) from dn (..., cols): dx in out_dtype or, where the kernel has no
     such pair of types, fp32."""
     rows, cols = q.shape
@@ -338,18 +360,21 @@ def _norm_ckpt_bwd(dn, dh, weight, q, stats, shape, out_dtype, want_dw):
     dx_dtype = dn.dtype if out_dtype == dn.dtype else torch.float32
     if dh is not None and dh.dtype != dx_dtype:
         dh = dh.to(dx_dtype)
-    dn2 = _rows2(dn)
-    dh2 = None if dh is None else _rows2(dh)
-    dx = torch.empty(shape, dtype=dx_dtype, device=dev)
-    dw = work = None
+    dn2, lddn = _lines(dn, cols)
+    hp, lddh = None, cols
+    if dh is not None:
+        dh2, lddh = _lines(dh, cols)
+        hp = dh2.data_ptr()
+    dx = _like(dn, dx_dtype)
+    dw = wp = kp = None
     if want_dw:
         dw = torch.empty(cols, dtype=torch.float32, device=dev)
         work = torch.empty(_bwd_floats(rows, cols), dtype=torch.float32, device=dev)
+        wp, kp = dw.data_ptr(), work.data_ptr()
     sp = stats.data_ptr()
-    _call("mmb_norm_ck8_bwd", idx, rows, cols, _TYPES[dn.dtype], dn2.data_ptr(), _ld(dn2),
-          _TYPES[dx_dtype], _p(dh2), cols if dh2 is None else _ld(dh2),
-          _p(_weight(weight, cols)), q.data_ptr(), _ld(q), sp, sp + 4 * rows * -(-cols // GROUP),
-          dx.data_ptr(), cols, _p(dw), _p(work))
+    _call("mmb_norm_ck8_bwd", idx, rows, cols, _TYPES[dn.dtype], dn2.data_ptr(), lddn,
+          _TYPES[dx_dtype], hp, lddh, _p(_weight(weight, cols)), q.data_ptr(), q.stride(0), sp,
+          sp + 4 * rows * -(-cols // GROUP), dx.data_ptr(), cols, wp, kp)
     return dx, dw
 
 
@@ -363,21 +388,21 @@ class RmsNormCkptFn(torch.autograd.Function):
         n, h, q, stats = _norm_ckpt(x, weight, residual, eps, 1, n_dtype,
                                     any(ctx.needs_input_grad[:3]), "rms_norm_ckpt")
         ctx.save_for_backward(weight, q, stats)
-        ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype)
+        ctx.meta = (x.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         return (n, h) if h is not None else n
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dn, dh=None):
-        shape, xdt, rdt = ctx.meta
+        xdt, rdt = ctx.meta
         need_x, need_w, need_r = ctx.needs_input_grad[:3]
         weight, q, stats = ctx.saved_tensors
         dw = None
         if dn is None:
             dx = dh
         else:
-            dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, stats, shape, rdt or xdt, need_w)
+            dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, stats, rdt or xdt, need_w)
         return (_as(dx, xdt) if need_x else None, None if dw is None else _as(dw, weight.dtype),
                 _as(dx, rdt) if need_r else None, None, None)
 
@@ -476,7 +501,7 @@ class NormLinearCkptFn(torch.autograd.Function):
                                     any(ctx.needs_input_grad[:5]), "norm_linear_ckpt")
         y = _linear(n, weight, bias)
         ctx.save_for_backward(norm_weight, weight, q, stats)
-        ctx.meta = (x.shape, x.dtype, None if residual is None else residual.dtype,
+        ctx.meta = (x.dtype, None if residual is None else residual.dtype,
                     None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
         return (y, h) if h is not None else y
@@ -484,7 +509,7 @@ class NormLinearCkptFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dy, dh=None):
-        shape, xdt, rdt, bdt = ctx.meta
+        xdt, rdt, bdt = ctx.meta
         need = ctx.needs_input_grad
         norm_weight, weight, q, stats = ctx.saved_tensors
         if dy is None:
@@ -494,7 +519,7 @@ class NormLinearCkptFn(torch.autograd.Function):
         if need[0] or need[1] or need[2]:
             with torch.autocast("cuda", enabled=False):
                 dn = torch.matmul(dy, weight.to(dy.dtype))
-            dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, shape, rdt or xdt, need[1])
+            dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, rdt or xdt, need[1])
         if need[3]:
             sp, nw = stats.data_ptr(), _weight(norm_weight, cols)
             dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, sp,
