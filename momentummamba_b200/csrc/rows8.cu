@@ -111,9 +111,12 @@ struct T8F16 {
 };
 
 // Column of value j of this lane in the 256-column chunk at c0.
+constexpr __host__ __device__ __forceinline__ int r8_off(int j) {
+    return (j >> 2) * R8_GROUP + (j & 3) * 32;
+}
 template <bool VEC>
 __device__ __forceinline__ int64_t r8_col(int64_t c0, int lane, int j) {
-    return VEC ? c0 + lane * 8 + j : c0 + (j >> 2) * R8_GROUP + (j & 3) * 32 + lane;
+    return VEC ? c0 + lane * 8 + j : c0 + r8_off(j) + lane;
 }
 
 // 8 values of a row, zeros past its end.  Raw form first, so that all of a
@@ -136,10 +139,15 @@ struct R8Load<E, false> {
     typename E::T r[8];
     __device__ __forceinline__ void load(const typename E::T* row, int64_t c0, int lane,
                                          int64_t cols) {
+        // whole chunks (all but a row's last) without a comparison a value
+        const typename E::T* q = row + c0 + lane;
+        const int left = (int)(cols - c0) - lane;
+        if (cols - c0 >= R8_CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = r8_col<false>(c0, lane, j);
-            r[j] = c < cols ? row[c] : E::from_f(0.f);
+            for (int j = 0; j < 8; ++j) r[j] = q[r8_off(j)];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = r8_off(j) < left ? q[r8_off(j)] : E::from_f(0.f);
         }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -153,10 +161,15 @@ __device__ __forceinline__ void r8_store(typename E::T* row, int64_t c0, int lan
     if constexpr (VEC) {
         if (c0 + lane * 8 < cols) E::stv(row + c0 + lane * 8, v);
     } else {
+        typename E::T* q = row + c0 + lane;
+        const int left = (int)(cols - c0) - lane;
+        if (cols - c0 >= R8_CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = r8_col<false>(c0, lane, j);
-            if (c < cols) row[c] = E::from_f(v[j]);
+            for (int j = 0; j < 8; ++j) q[r8_off(j)] = E::from_f(v[j]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (r8_off(j) < left) q[r8_off(j)] = E::from_f(v[j]);
         }
     }
 }
@@ -177,10 +190,15 @@ __device__ __forceinline__ void r8_store_q(int8_t* row, int64_t c0, int lane, in
             *reinterpret_cast<uint2*>(row + c0 + lane * 8) =
                 make_uint2(r8_pack4(b[0], b[1], b[2], b[3]), r8_pack4(b[4], b[5], b[6], b[7]));
     } else {
+        int8_t* q = row + c0 + lane;
+        const int left = (int)(cols - c0) - lane;
+        if (cols - c0 >= R8_CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = r8_col<false>(c0, lane, j);
-            if (c < cols) row[c] = (int8_t)(b[j] & 0xff);
+            for (int j = 0; j < 8; ++j) q[r8_off(j)] = (int8_t)b[j];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (r8_off(j) < left) q[r8_off(j)] = (int8_t)b[j];
         }
     }
 }
@@ -208,10 +226,14 @@ template <>
 struct R8LoadQ<false> {
     int8_t r[8];
     __device__ __forceinline__ void load(const int8_t* row, int64_t c0, int lane, int64_t cols) {
+        const int8_t* q = row + c0 + lane;
+        const int left = (int)(cols - c0) - lane;
+        if (cols - c0 >= R8_CHUNK) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t c = r8_col<false>(c0, lane, j);
-            r[j] = c < cols ? row[c] : (int8_t)0;
+            for (int j = 0; j < 8; ++j) r[j] = q[r8_off(j)];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) r[j] = r8_off(j) < left ? q[r8_off(j)] : (int8_t)0;
         }
     }
     __device__ __forceinline__ void get(float (&v)[8]) const {
@@ -652,7 +674,9 @@ static R8Shape r8_shape(int64_t cols, bool vec) {
     if (vec && cols <= 128) return {1, 1, 8, true};
     if (chunks <= 1) return {1, 1, 4};
     if (chunks <= 2) return {1, 2, 4};
-    if (chunks <= 4) return {1, 4, 4};
+    // single loads of four chunks take a thread 242 registers in the backward: two
+    // warps a row then (65536 x 1001 fp16)
+    if (chunks <= 4) return vec ? R8Shape{1, 4, 4} : R8Shape{2, 2, 1};
     // several warps a row: two chunks each as long as 16 warps suffice (four leave
     // a 512-thread block too few registers)
     if (chunks <= 2 * R8_MAX_WARPS) return {(int)((chunks + 1) / 2), 2, 1};
@@ -723,7 +747,9 @@ static int r8_fwd_check(const R8Fwd& p, int xt, int rt) {
 // partial sums stay small.
 static int r8_bwd_blocks(int64_t rows, const R8Shape& s) {
     const int64_t need = (rows + s.rows - 1) / s.rows;
-    const int64_t most = 148 * (s.warps == 1 ? 4 : s.warps <= 8 ? 2 : 1);
+    // as many as are resident at once: a fourth block of 128 threads an SM waited for
+    // the others to end (65536 x 1024 bf16: 133 us)
+    const int64_t most = 148 * (s.rows > 1 ? 3 : s.warps < 16 ? 16 / s.warps : 1);
     return (int)min64(need, most);
 }
 template <class EN, class EX, bool VEC>
@@ -738,7 +764,7 @@ static int r8_bwd_launch(const R8Bwd& p, const R8Shape& s, int blocks, cudaStrea
     if (s.nc == 1) r8_bwd_kernel<EN, EX, VEC, 1, 4, 128><<<blocks, block, sm, st>>>(p);
     else if (s.nc == 2 && s.warps == 1)
         r8_bwd_kernel<EN, EX, VEC, 2, 2, 128><<<blocks, block, sm, st>>>(p);
-    else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, 1, 512><<<blocks, block, sm, st>>>(p);
+    else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, VEC ? 2 : 1, 512><<<blocks, block, sm, st>>>(p);
     else if (s.warps == 1) r8_bwd_kernel<EN, EX, VEC, 4, 1, 128><<<blocks, block, sm, st>>>(p);
     else r8_bwd_kernel<EN, EX, VEC, 4, 1, 512><<<blocks, block, sm, st>>>(p);
     return mmb_launch_status();
