@@ -17,6 +17,13 @@ CUDA kernels; there is no CPU path:
   "sequential"
       the row-scan kernel of momentum_scan_cuda on the materialised tensors.
 
+``act_ckpt="int8"`` (training): each block keeps the inputs of its two large
+projections as 8-bit checkpoints.  The residual's addition, the norm and in_proj
+are one autograd step (int8.norm_linear_ckpt) whose backward reads a single 8-bit
+copy of the sum, and out_proj keeps its input in 8 bits (int8.linear_ckpt);
+outputs are those of the plain path, gradients differ by the kept values'
+rounding (half a step of 1/64 to 1/127 of a group's largest value).
+
 In every mode the block's causal depthwise conv1d + SiLU is one kernel
 (conv.conv1d_silu, no transposes), and ``step()`` runs the conv-cache update
 and the state update (with the dt softplus and the SiLU(z) gate) as one kernel
@@ -33,6 +40,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .conv import conv1d_silu, conv1d_step, mmscan_step
+from .int8 import linear_ckpt, norm_linear_ckpt
 from .momentum_scan_cuda import momentum_scan_cuda
 from .pscan import pscan
 from .selective_scan import selective_scan_momentum_fn
@@ -73,7 +81,11 @@ class MambaMomentumConfig:
     pscan: bool = True
     pscan_mode: str = "cuda_sequential"
 
+    act_ckpt: str = "none"  # "int8": projections' inputs kept in 8 bits for the backward
+
     def __post_init__(self):
+        if self.act_ckpt not in ("none", "int8"):
+            raise ValueError(f"act_ckpt must be 'none' or 'int8', got {self.act_ckpt!r}")
         self.d_inner = self.expand_factor * self.d_model
         if self.dt_rank == "auto":
             self.dt_rank = math.ceil(self.d_model / 16)
@@ -101,6 +113,11 @@ class MambaMomentum(nn.Module):
         self.layers = nn.ModuleList([ResidualBlock(config) for _ in range(config.n_layers)])
 
     def forward(self, x):
+        if self.config.act_ckpt == "int8" and self.config.n_layers:
+            h = None
+            for layer in self.layers:  # each layer adds its predecessor's output to the stream
+                x, h = layer.forward_ckpt(x, h)
+            return x + h
         for layer in self.layers:
             x = layer(x)
         return x
@@ -118,7 +135,21 @@ class ResidualBlock(nn.Module):
         self.norm = RMSNorm(config.d_model, config.rms_norm_eps, config.mup)
 
     def forward(self, x):
+        if self.mixer.config.act_ckpt == "int8":
+            out, h = self.forward_ckpt(x, None)
+            return out + h
         return self.mixer(self.norm(x)) + x
+
+    def forward_ckpt(self, x, residual):
+        """(mixer(norm(h)), h) of h = x + residual (x where residual is None), with the
+        projections' inputs kept in 8 bits."""
+        m = self.mixer
+        if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+            residual = residual.float()
+        xz, h = norm_linear_ckpt(x, None if self.norm.use_mup else self.norm.weight,
+                                 m.in_proj.weight, m.in_proj.bias, residual=residual,
+                                 eps=self.norm.eps)
+        return linear_ckpt(m.mix(xz), m.out_proj.weight, m.out_proj.bias), h
 
     def step(self, x, cache):
         out, cache = self.mixer.step(self.norm(x), cache)
@@ -182,14 +213,15 @@ class MambaMomentumBlock(nn.Module):
         return conv1d_silu(x, self.conv1d.weight, self.conv1d.bias)
 
     def forward(self, x):
-        xz = self.in_proj(x)
+        return self.out_proj(self.mix(self.in_proj(x)))
+
+    def mix(self, xz):
+        """What lies between the block's projections: conv, scan and gate."""
         x, z = xz.chunk(2, dim=-1)
         x = self._conv_silu(x)
         if self.config.pscan and self.config.pscan_mode in _FUSED_MODES:
-            y = self._ssm_fused(x, z)
-        else:
-            y = self.ssm_momentum(x) * F.silu(z)
-        return self.out_proj(y)
+            return self._ssm_fused(x, z)
+        return self.ssm_momentum(x) * F.silu(z)
 
     def _project(self, x):
         A = -torch.exp(self.A_log.float())

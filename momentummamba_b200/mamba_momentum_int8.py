@@ -1,0 +1,92 @@
+"""MambaMomentum served in 8 bits: the two large projections of every block on
+linear_q8, their weights quantised once per output channel, their inputs per token.
+
+    model8 = Int8MambaMomentum(model)          # model: a trained MambaMomentum
+    y = model8(x)                              # (batch, length, d_model)
+    y, caches = model8.step(x, caches)         # one token, caches as MambaMomentum.step's
+
+Between the blocks only the residual stream is stored in full: each block adds
+its predecessor's output to it, norms the sum and emits 8-bit rows in one kernel
+(rms_norm_q8).  The conv, the scan and the two small projections (x_proj,
+dt_proj: the recurrence's step sizes and B, C, which 8 bits would disturb most)
+run as in the model, on its parameters.  The weights held in 8 bits take a
+quarter of their fp32 size; a decoding step reads little else.
+
+No reference counterpart (the reference serves in fp32).  Inference only: no
+gradients.
+"""
+from __future__ import annotations
+
+import torch
+import torch.nn as nn
+
+from .conv import conv1d_step
+from .int8 import Q8Rows, linear_q8, quantize_rows, rms_norm_q8
+from .mamba_momentum import MambaMomentum, MambaMomentumBlock
+
+
+class Int8Linear(nn.Module):
+    """A linear's weight as 8-bit rows (one scale an output channel) and its bias."""
+
+    def __init__(self, linear: nn.Linear):
+        super().__init__()
+        w = quantize_rows(linear.weight.detach())
+        self.register_buffer("q", w.q)
+        self.register_buffer("scale", w.scale)
+        self.register_buffer("bias", None if linear.bias is None
+                             else linear.bias.detach().float().clone())
+
+    def forward(self, x: Q8Rows, out_dtype: torch.dtype) -> torch.Tensor:
+        return linear_q8(x, Q8Rows(self.q, self.scale), self.bias, out_dtype=out_dtype)
+
+
+class Int8Block(nn.Module):
+    """One residual block; holds the model's own mixer for what stays in full."""
+
+    def __init__(self, norm, mixer: MambaMomentumBlock):
+        super().__init__()
+        self.norm, self.mixer = norm, mixer
+        self.in_proj, self.out_proj = Int8Linear(mixer.in_proj), Int8Linear(mixer.out_proj)
+
+    def _in(self, x, residual):
+        n, h = rms_norm_q8(x, None if self.norm.use_mup else self.norm.weight, residual=residual,
+                           eps=self.norm.eps)
+        return self.in_proj(n, self.mixer.x_proj.weight.dtype), h
+
+    def _out(self, y):
+        return self.out_proj(quantize_rows(y), self.mixer.x_proj.weight.dtype)
+
+    def forward(self, x, residual):
+        xz, h = self._in(x, residual)
+        return self._out(self.mixer.mix(xz)), h
+
+    def step(self, x, residual, cache):
+        h_state, v_state, inputs = cache
+        xz, h = self._in(x, residual)
+        x, z = xz.chunk(2, dim=1)
+        conv = self.mixer.conv1d
+        x, inputs = conv1d_step(x, inputs, conv.weight, conv.bias)
+        y, h_state, v_state = self.mixer._ssm_step(x, h_state, v_state, z)
+        return self._out(y), h, (h_state, v_state, inputs)
+
+
+class Int8MambaMomentum(nn.Module):
+    def __init__(self, model: MambaMomentum):
+        super().__init__()
+        self.config = model.config
+        self.layers = nn.ModuleList([Int8Block(b.norm, b.mixer) for b in model.layers])
+
+    @torch.no_grad()
+    def forward(self, x):
+        h = None
+        for layer in self.layers:
+            x, h = layer(x, h)
+        return x if h is None else x + h
+
+    @torch.no_grad()
+    def step(self, x, caches):
+        """One token x (batch, d_model) through every layer; caches is updated in place."""
+        h = None
+        for i, layer in enumerate(self.layers):
+            x, h, caches[i] = layer.step(x, h, caches[i])
+        return (x if h is None else x + h), caches
