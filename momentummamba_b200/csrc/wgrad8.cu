@@ -550,22 +550,39 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     }
 }
 
-// dw[n, k] = col[k] * sum of the slices' [n, k], in order; 4 columns a thread
-__global__ void __launch_bounds__(256)
+// dw[n, k] = col[k] * sum of the slices' [n, k]: 4 columns a thread (blockDim.x of
+// them a block), the slices dealt to blockDim.y groups of threads, always in the
+// same order.  Many slices of a small result take 8 groups (37 slices of 512 x 128:
+// 6.7 -> 3.6 us), few slices of a large one take 1 (2 of 4096 x 1024: 46 -> 10 us).
+constexpr int W8_SUM_NT = 256, W8_SUM_GROUPS = 8;
+__global__ void __launch_bounds__(W8_SUM_NT)
     w8_sum_kernel(int64_t N, int64_t K, const float* __restrict__ work, int64_t ldp,
                   int64_t slices, const float* __restrict__ col, void* dw, int64_t ldw,
                   int out_type) {
-    const int64_t quads = ldp / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * quads) return;
-    const int64_t n = i / quads, k = (i % quads) * 4;
+    __shared__ float4 s[W8_SUM_NT];
+    const int qi = threadIdx.x, zi = threadIdx.y, nq = blockDim.x, nz = blockDim.y;
+    const int64_t quads = ldp / 4, i = (int64_t)blockIdx.x * nq + qi;
+    const bool in = i < N * quads;
+    const int64_t n = in ? i / quads : 0, k = in ? (i % quads) * 4 : 0;
     const float* w = work + n * ldp + k;
     float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int64_t z = 0; z < slices; ++z) {
-        const float4 v = *reinterpret_cast<const float4*>(w + z * N * ldp);
-        t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+    if (in) {
+#pragma unroll 4
+        for (int64_t z = zi; z < slices; z += nz) {
+            const float4 v = *reinterpret_cast<const float4*>(w + z * N * ldp);
+            t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+        }
     }
+    if (nz > 1) {
+        s[zi * nq + qi] = t;
+        __syncthreads();
+        if (zi) return;
+        for (int g = 1; g < nz; ++g) {
+            const float4 v = s[g * nq + qi];
+            t.x += v.x; t.y += v.y; t.z += v.z; t.w += v.w;
+        }
+    }
+    if (!in) return;
     const float v[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -640,8 +657,10 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     const int rc = mmb_launch_status();
     if (rc != MMB_OK || p.slices == 1) return rc;
     const int64_t quads = p.N * (p.ldp / 4);
-    w8_sum_kernel<<<(unsigned)((quads + 255) / 256), 256, 0, s>>>(p.N, p.K, p.work, p.ldp, p.slices,
-                                                                  p.col, p.dw, p.ldw, p.out_type);
+    const unsigned groups = p.slices >= 2 * W8_SUM_GROUPS ? W8_SUM_GROUPS : 1;
+    const unsigned nq = W8_SUM_NT / groups;
+    w8_sum_kernel<<<(unsigned)((quads + nq - 1) / nq), dim3(nq, groups), 0, s>>>(
+        p.N, p.K, p.work, p.ldp, p.slices, p.col, p.dw, p.ldw, p.out_type);
     return mmb_launch_status();
 }
 

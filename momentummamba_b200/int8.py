@@ -50,7 +50,7 @@ _get_device = torch._C._cuda_getDevice
 def _type(t: torch.Tensor, what: str) -> int:
     code = _TYPES.get(t.dtype)
     if code is None:
-        raise ValueError(f"{what} must be fp32, bf16 or fp16, got {t.dtype}")
+        raise ValueError(f"{what}: tensors must be fp32, bf16 or fp16, got {t.dtype}")
     return code
 
 
@@ -139,20 +139,22 @@ def _empty_q(rows: int, cols: int, device) -> torch.Tensor:
                                device=device)
 
 
-def _check_rows(x: torch.Tensor, residual: Optional[torch.Tensor], what: str) -> int:
-    if x.dim() < 1 or x.shape[-1] < 1:
+def _check_rows(x: torch.Tensor, shape, residual: Optional[torch.Tensor], what: str) -> int:
+    """The width of x's rows, checked with the residual's shape and type."""
+    if not shape or shape[-1] < 1:
         raise ValueError(f"{what}: x must have a last dimension of one or more")
-    cols = x.shape[-1]
+    cols = shape[-1]
     if cols > MAX_COLS:
         raise ValueError(f"{what}: rows of more than {MAX_COLS} values are not supported, "
                          f"got {cols}")
     if residual is not None:
-        if residual.shape != x.shape:
-            raise ValueError(f"{what}: x and residual must share a shape, got {tuple(x.shape)} "
+        if residual.shape != shape:
+            raise ValueError(f"{what}: x and residual must share a shape, got {tuple(shape)} "
                              f"and {tuple(residual.shape)}")
-        if residual.dtype != x.dtype and residual.dtype != torch.float32:
+        rd = residual.dtype
+        if rd is not torch.float32 and rd is not x.dtype:
             raise ValueError(f"{what}: the residual must be of x's type or fp32, got "
-                             f"{residual.dtype} with x {x.dtype}")
+                             f"{rd} with x {x.dtype}")
     return cols
 
 
@@ -198,6 +200,13 @@ class Ckpt8:
         return _restore(self.q, self.scale, True, dtype).view(self.shape)
 
 
+def _made(cls, q, scale):
+    """Rows that a kernel has just made: nothing of them is left to check."""
+    r = cls.__new__(cls)
+    r.q, r.scale = q, scale
+    return r
+
+
 def _restore(q, scale, grouped, dtype):
     idx = _index(q, scale)
     code = _out_type(dtype)
@@ -214,8 +223,9 @@ def _restore(q, scale, grouped, dtype):
 
 def _norm_q8(x, weight, residual, eps, norm, what):
     idx = _index(x, weight, residual)
-    xt = rt = _type(x, what + ": x")
-    cols = _check_rows(x, residual, what)
+    xt = rt = _type(x, what)
+    shape = x.shape
+    cols = _check_rows(x, shape, residual, what)
     weight = _weight(weight, cols)
     x2, ldx = _lines(x, cols)
     rows, dev = x.numel() // cols, x.device
@@ -227,14 +237,14 @@ def _norm_q8(x, weight, residual, eps, norm, what):
         h = _like(residual, residual.dtype)
         rp, hp = r2.data_ptr(), h.data_ptr()
     q = _empty_q(rows, cols, dev)
-    scale = torch.empty(*x.shape[:-1], dtype=torch.float32, device=dev) if x.dim() > 1 else \
-        torch.empty((), dtype=torch.float32, device=dev)
+    scale = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows:
         _call("mmb_norm_q8", idx, rows, cols, xt, x2.data_ptr(), ldx, rt, rp, ldr, _p(weight),
               eps, norm, hp, cols, q.data_ptr(), q.stride(0), scale.data_ptr())
-    if x.dim() != 2:
-        q = q.unflatten(0, x.shape[:-1]) if x.dim() > 2 else q[0]
-    return Q8Rows(q, scale), h
+    if len(shape) != 2:
+        q = q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]
+        scale = scale.view(shape[:-1])
+    return _made(Q8Rows, q, scale), h
 
 
 def rms_norm_q8(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -306,8 +316,8 @@ def _norm_ckpt(x, weight, residual, eps, norm, n_dtype, keep, what):
     """(n, h, q, stats) of one mmb_norm_ck8_fwd call.  stats: the groups' scales and,
     with norm, one rstd a row behind them, in one fp32 tensor."""
     idx = _index(x, weight, residual)
-    xt = rt = _type(x, what + ": x")
-    cols = _check_rows(x, residual, what)
+    xt = rt = _type(x, what)
+    cols = _check_rows(x, x.shape, residual, what)
     weight = _weight(weight, cols)
     x2, ldx = _lines(x, cols)
     rows, dev = x.numel() // cols, x.device
@@ -338,7 +348,10 @@ def _norm_ckpt(x, weight, residual, eps, norm, n_dtype, keep, what):
 def checkpoint_rows(x: torch.Tensor) -> Ckpt8:
     """x (..., cols) kept in 8 bits (fp32, bf16 or fp16 in)."""
     _, _, q, stats = _norm_ckpt(x, None, None, 0.0, 0, None, True, "checkpoint_rows")
-    return Ckpt8(q, stats.view(q.shape[0], -(-q.shape[1] // GROUP)), x.shape)
+    kept = _made(Ckpt8, q, stats.view(q.shape[0], -1) if q.shape[0] else
+                 stats.view(0, -(-q.shape[1] // GROUP)))
+    kept.shape = x.shape
+    return kept
 
 
 @lru_cache(maxsize=256)
@@ -382,29 +395,42 @@ def _as(t: Optional[torch.Tensor], dtype) -> Optional[torch.Tensor]:
     return t if t is None or t.dtype == dtype else t.to(dtype)
 
 
+def _backward_of(impl):
+    """backward that impl computes once: a second derivative raises.  The wrapper that
+    says so costs 6 us, and matters only where the backward itself is recorded."""
+    guarded = once_differentiable(impl)
+
+    def backward(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else impl)(ctx, *grads)
+
+    return staticmethod(backward)
+
+
+def _rms_norm_ckpt_bwd(ctx, dn, dh=None):
+    xdt, rdt = ctx.meta
+    need_x, need_w, need_r = ctx.needs_input_grad[:3]
+    (weight,) = ctx.saved_tensors
+    dw = None
+    if dn is None:
+        dx = dh
+    else:
+        dx, dw = _norm_ckpt_bwd(dn, dh, weight, ctx.q, ctx.stats, rdt or xdt, need_w)
+    return (_as(dx, xdt) if need_x else None, None if dw is None else _as(dw, weight.dtype),
+            _as(dx, rdt) if need_r else None, None, None)
+
+
 class RmsNormCkptFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, residual, eps, n_dtype):
         n, h, q, stats = _norm_ckpt(x, weight, residual, eps, 1, n_dtype,
                                     any(ctx.needs_input_grad[:3]), "rms_norm_ckpt")
-        ctx.save_for_backward(weight, q, stats)
+        ctx.save_for_backward(weight)
+        ctx.q, ctx.stats = q, stats
         ctx.meta = (x.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         return (n, h) if h is not None else n
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dn, dh=None):
-        xdt, rdt = ctx.meta
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        weight, q, stats = ctx.saved_tensors
-        dw = None
-        if dn is None:
-            dx = dh
-        else:
-            dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, stats, rdt or xdt, need_w)
-        return (_as(dx, xdt) if need_x else None, None if dw is None else _as(dw, weight.dtype),
-                _as(dx, rdt) if need_r else None, None, None)
+    backward = _backward_of(_rms_norm_ckpt_bwd)
 
 
 def rms_norm_ckpt(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
@@ -469,7 +495,7 @@ def weight_grad_ckpt(dy: torch.Tensor, kept: Ckpt8, row_scale: Optional[torch.Te
     one.  In dy's type unless out_dtype says otherwise; sums are fp32."""
     q, scale = kept.q, kept.scale
     idx = _index(dy, q, scale, row_scale, col_scale)
-    code = _type(dy, "weight_grad_ckpt: dy")
+    code = _type(dy, "weight_grad_ckpt")
     M, K = q.shape
     if dy.dim() < 1 or dy.shape[-1] < 1 or dy.numel() != M * dy.shape[-1]:
         raise ValueError(f"weight_grad_ckpt: dy (..., N) must have the checkpoint's {M} rows, got "
@@ -493,6 +519,31 @@ def _linear(n, weight, bias):
         return torch.nn.functional.linear(n, weight.to(dt), None if bias is None else bias.to(dt))
 
 
+def _norm_linear_ckpt_bwd(ctx, dy, dh=None):
+    xdt, rdt, bdt = ctx.meta
+    need = ctx.needs_input_grad
+    norm_weight, weight = ctx.saved_tensors
+    q, stats = ctx.q, ctx.stats
+    if dy is None:
+        return _as(dh, xdt), None, _as(dh, rdt) if need[2] else None, None, None, None
+    rows, cols = q.shape
+    dx = dnw = dw = db = None
+    if need[0] or need[1] or need[2]:
+        with torch.autocast("cuda", enabled=False):
+            dn = torch.matmul(dy, weight.to(dy.dtype))
+        dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, rdt or xdt, need[1])
+    if need[3]:
+        sp, nw = stats.data_ptr(), _weight(norm_weight, cols)
+        dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, sp,
+                          sp + 4 * rows * -(-cols // GROUP), _p(nw), weight.dtype,
+                          _out_type(weight.dtype))
+    if need[4] and bdt is not None:
+        db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
+    return (_as(dx, xdt) if need[0] else None,
+            None if dnw is None else _as(dnw, norm_weight.dtype),
+            _as(dx, rdt) if need[2] else None, dw, db, None)
+
+
 class NormLinearCkptFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, norm_weight, residual, weight, bias, eps):
@@ -500,36 +551,14 @@ class NormLinearCkptFn(torch.autograd.Function):
         n, h, q, stats = _norm_ckpt(x, norm_weight, residual, eps, 1, dt,
                                     any(ctx.needs_input_grad[:5]), "norm_linear_ckpt")
         y = _linear(n, weight, bias)
-        ctx.save_for_backward(norm_weight, weight, q, stats)
+        ctx.save_for_backward(norm_weight, weight)
+        ctx.q, ctx.stats = q, stats
         ctx.meta = (x.dtype, None if residual is None else residual.dtype,
                     None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
         return (y, h) if h is not None else y
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dh=None):
-        xdt, rdt, bdt = ctx.meta
-        need = ctx.needs_input_grad
-        norm_weight, weight, q, stats = ctx.saved_tensors
-        if dy is None:
-            return _as(dh, xdt), None, _as(dh, rdt) if need[2] else None, None, None, None
-        rows, cols = q.shape
-        dx = dnw = dw = db = None
-        if need[0] or need[1] or need[2]:
-            with torch.autocast("cuda", enabled=False):
-                dn = torch.matmul(dy, weight.to(dy.dtype))
-            dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, rdt or xdt, need[1])
-        if need[3]:
-            sp, nw = stats.data_ptr(), _weight(norm_weight, cols)
-            dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, sp,
-                              sp + 4 * rows * -(-cols // GROUP), _p(nw), weight.dtype,
-                              _out_type(weight.dtype))
-        if need[4] and bdt is not None:
-            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
-        return (_as(dx, xdt) if need[0] else None,
-                None if dnw is None else _as(dnw, norm_weight.dtype),
-                _as(dx, rdt) if need[2] else None, dw, db, None)
+    backward = _backward_of(_norm_linear_ckpt_bwd)
 
 
 def norm_linear_ckpt(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weight: torch.Tensor,
@@ -545,32 +574,35 @@ def norm_linear_ckpt(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weigh
     return out if residual is not None else (out, x)
 
 
+def _linear_ckpt_bwd(ctx, dy):
+    xdt, bdt = ctx.meta
+    need = ctx.needs_input_grad
+    (weight,) = ctx.saved_tensors
+    q, stats = ctx.q, ctx.stats
+    dx = dw = db = None
+    if need[0]:
+        with torch.autocast("cuda", enabled=False):
+            dx = _as(torch.matmul(dy, weight.to(dy.dtype)), xdt)
+    if need[1]:
+        dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, stats.data_ptr(), None,
+                          None, weight.dtype, _out_type(weight.dtype))
+    if need[2] and bdt is not None:
+        db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
+    return dx, dw, db
+
+
 class LinearCkptFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         q = stats = None
         if ctx.needs_input_grad[1]:
             _, _, q, stats = _norm_ckpt(x, None, None, 0.0, 0, None, True, "linear_ckpt")
-        ctx.save_for_backward(weight, q, stats)
+        ctx.save_for_backward(weight)
+        ctx.q, ctx.stats = q, stats
         ctx.meta = (x.dtype, None if bias is None else bias.dtype)
         return _linear(x.to(_linear_types(weight.dtype)), weight, bias)
 
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        xdt, bdt = ctx.meta
-        need = ctx.needs_input_grad
-        weight, q, stats = ctx.saved_tensors
-        dx = dw = db = None
-        if need[0]:
-            with torch.autocast("cuda", enabled=False):
-                dx = _as(torch.matmul(dy, weight.to(dy.dtype)), xdt)
-        if need[1]:
-            dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, stats.data_ptr(), None,
-                              None, weight.dtype, _out_type(weight.dtype))
-        if need[2] and bdt is not None:
-            db = dy.reshape(-1, dy.shape[-1]).sum(0, dtype=torch.float32).to(bdt)
-        return dx, dw, db
+    backward = _backward_of(_linear_ckpt_bwd)
 
 
 def linear_ckpt(x: torch.Tensor, weight: torch.Tensor,
@@ -582,7 +614,7 @@ def linear_ckpt(x: torch.Tensor, weight: torch.Tensor,
 
 def _linear_check(x, weight, bias, what):
     _lib.require_cuda(x, weight, bias)
-    _type(weight, what + ": weight")
+    _type(weight, what)
     if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
         raise ValueError(f"{what}: x (..., K) and weight (N, K) must share K, got {tuple(x.shape)} "
                          f"and {tuple(weight.shape)}")
