@@ -382,6 +382,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 const int s = rl.s, cs = rc.s;
                 ok = ws_wait(&free_c[cs], rc.ph ^ 1u, abort, p.err) &&
                      ws_wait(&full[s], rl.ph, abort, p.err);
+                ok = __all_sync(0xffffffffu, ok);  // a warp leaves together
                 if (!ok) break;
                 const uint32_t fs = smem_u32(slot_f(s)), qs = smem_u32(slot_q(s)) + piece * 16;
                 const uint32_t as = smem_u32(slot_a(cs));
@@ -607,14 +608,17 @@ static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
     const double tile_us = 1.0 + D::AG * (D::F32 ? 0.5 : 1.0);
     const double slice_us = 2.0 * (double)N * (double)K * 4.0 / 5e6;
     W8Plan best{1, nblk, 1e30};
-    for (int64_t s = 1; s <= nblk && s <= 148; ++s) {
+    const auto consider = [&](int64_t s) {
+        s = s < 1 ? 1 : s > nblk ? nblk : s;
         const int64_t per = (nblk + s - 1) / s;
-        if ((nblk + per - 1) / per != s) continue;  // the same as a smaller count
+        s = (nblk + per - 1) / per;  // the slices that this many blocks each make
         const int64_t rounds = (tiles * s + 147) / 148;
         const double t = (double)rounds * ((double)per * block_us + tile_us) +
                          (s > 1 ? 2.0 + (double)s * slice_us : 0.0);
         if (t < best.us) best = {s, per, t};
-    }
+    };
+    for (int64_t r = 1; r <= 4; ++r) consider(148 * r / tiles);  // r full rounds of the SMs
+    for (int64_t s = 1; s <= 128; s *= 2) consider(s);
     return best;
 }
 // 16-bit dy: one group a tile or two, whichever is estimated faster

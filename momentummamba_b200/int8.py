@@ -409,12 +409,12 @@ def _backward_of(impl):
 def _rms_norm_ckpt_bwd(ctx, dn, dh=None):
     xdt, rdt = ctx.meta
     need_x, need_w, need_r = ctx.needs_input_grad[:3]
-    (weight,) = ctx.saved_tensors
+    weight, q, stats = ctx.saved_tensors
     dw = None
     if dn is None:
         dx = dh
     else:
-        dx, dw = _norm_ckpt_bwd(dn, dh, weight, ctx.q, ctx.stats, rdt or xdt, need_w)
+        dx, dw = _norm_ckpt_bwd(dn, dh, weight, q, stats, rdt or xdt, need_w)
     return (_as(dx, xdt) if need_x else None, None if dw is None else _as(dw, weight.dtype),
             _as(dx, rdt) if need_r else None, None, None)
 
@@ -424,8 +424,7 @@ class RmsNormCkptFn(torch.autograd.Function):
     def forward(ctx, x, weight, residual, eps, n_dtype):
         n, h, q, stats = _norm_ckpt(x, weight, residual, eps, 1, n_dtype,
                                     any(ctx.needs_input_grad[:3]), "rms_norm_ckpt")
-        ctx.save_for_backward(weight)
-        ctx.q, ctx.stats = q, stats
+        ctx.save_for_backward(weight, q, stats)
         ctx.meta = (x.dtype, None if residual is None else residual.dtype)
         ctx.set_materialize_grads(False)
         return (n, h) if h is not None else n
@@ -522,8 +521,7 @@ def _linear(n, weight, bias):
 def _norm_linear_ckpt_bwd(ctx, dy, dh=None):
     xdt, rdt, bdt = ctx.meta
     need = ctx.needs_input_grad
-    norm_weight, weight = ctx.saved_tensors
-    q, stats = ctx.q, ctx.stats
+    norm_weight, weight, q, stats = ctx.saved_tensors
     if dy is None:
         return _as(dh, xdt), None, _as(dh, rdt) if need[2] else None, None, None, None
     rows, cols = q.shape
@@ -551,8 +549,7 @@ class NormLinearCkptFn(torch.autograd.Function):
         n, h, q, stats = _norm_ckpt(x, norm_weight, residual, eps, 1, dt,
                                     any(ctx.needs_input_grad[:5]), "norm_linear_ckpt")
         y = _linear(n, weight, bias)
-        ctx.save_for_backward(norm_weight, weight)
-        ctx.q, ctx.stats = q, stats
+        ctx.save_for_backward(norm_weight, weight, q, stats)
         ctx.meta = (x.dtype, None if residual is None else residual.dtype,
                     None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
@@ -577,8 +574,7 @@ def norm_linear_ckpt(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weigh
 def _linear_ckpt_bwd(ctx, dy):
     xdt, bdt = ctx.meta
     need = ctx.needs_input_grad
-    (weight,) = ctx.saved_tensors
-    q, stats = ctx.q, ctx.stats
+    weight, q, stats = ctx.saved_tensors
     dx = dw = db = None
     if need[0]:
         with torch.autocast("cuda", enabled=False):
@@ -597,8 +593,7 @@ class LinearCkptFn(torch.autograd.Function):
         q = stats = None
         if ctx.needs_input_grad[1]:
             _, _, q, stats = _norm_ckpt(x, None, None, 0.0, 0, None, True, "linear_ckpt")
-        ctx.save_for_backward(weight)
-        ctx.q, ctx.stats = q, stats
+        ctx.save_for_backward(weight, q, stats)
         ctx.meta = (x.dtype, None if bias is None else bias.dtype)
         return _linear(x.to(_linear_types(weight.dtype)), weight, bias)
 
