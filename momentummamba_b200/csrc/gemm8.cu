@@ -12,13 +12,21 @@
 //
 //  * g8_tile_kernel, for products that fill the GPU: persistent, one CTA per
 //    SM, 128 tokens x BN channels, roles in separate warps (producer, MMA
-//    issuer, four epilogue warps) over a ring of K blocks and two TMEM
+//    issuer, eight epilogue warps) over a ring of K blocks and two TMEM
 //    accumulators, so tile t + 1 accumulates while tile t is scaled and stored.
+//    B200: 16384 x 8192 x 4096, bf16 out: 376 us, 2.92e15 operations/s, 1.78 times
+//    the measured bf16 rate; bound by the tensor cores under the power cap (440 us
+//    back to back).  76800 x 1024 x 256, fp32 out: 57-63 us, 5.3-5.9 TB/s; bound by
+//    writing 315 MB (48 us alone).  Stores of 32 bytes a lane straight from registers
+//    took 92 us there (32 lines a store), boxes of 128-byte rows by TMA 63.
 //  * g8_split_kernel, for few tokens (a decoding step), where streaming the
 //    weights is all there is to do: the weights are the MMA's 128-row operand
 //    and MT tokens its columns, K is cut across the CTAs of a cluster, and the
 //    cluster adds its partial sums through distributed shared memory (integers:
-//    the order does not matter).
+//    the order does not matter).  B200: one token 4096 x 1024 4.6 us, 48 tokens
+//    2048 x 4096 7.1 us, 8 tokens 8192 x 8192 16 us (10 at the copy rate); bound by
+//    the latency of a launch, one trip to memory and the cluster's two barriers
+//    (about 4.5 us), then by HBM.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
