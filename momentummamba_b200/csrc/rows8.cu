@@ -370,8 +370,11 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
     int8_t* qr = p.q ? p.q + row * p.qs : nullptr;
 
     if constexpr (!CK) {
-        // rows whose largest value is below 2^-100 count as zero (127 / top stays finite)
-        const float inv = top >= R8_TINY && top < INFINITY ? __fdiv_rn(127.f, top) : 0.f;
+        // rows whose largest value is below 2^-100 count as zero (127 / top stays finite).
+        // The reciprocal times 127, each rounded: what an array library makes of 127 / top,
+        // so that a restatement there lands on the same side of every step
+        const float inv =
+            top >= R8_TINY && top < INFINITY ? __fmul_rn(__frcp_rn(top), 127.f) : 0.f;
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             uint32_t b[8];
