@@ -116,9 +116,9 @@ __device__ __forceinline__ void bulk_wait_read() {
 
 // Bounded wait on phase `parity` that also gives up when another role aborted.
 // A poll may suspend the thread for up to WS_HINT_NS: waiting warps that poll
-// without one take most of the SM's issue slots from those that work (a third of
-// all instructions in the weight-gradient kernel were polls).  WS_POLLS of them
-// take about two seconds.
+// without one take issue slots from those that work (over a third of all
+// instructions in the weight-gradient kernel were polls).  WS_POLLS of them take
+// about two seconds.
 constexpr uint32_t WS_HINT_NS = 20000;
 constexpr int WS_POLLS = 100000;
 __device__ __forceinline__ bool mbar_try_wait_hint(uint64_t* bar, uint32_t parity) {
@@ -171,8 +171,7 @@ __device__ __forceinline__ void sts8(uint32_t a, uint32_t x, uint32_t y) {
     asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(a), "r"(x), "r"(y) : "memory");
 }
 
-// One arrival for a whole warp: 256 threads that arrive one by one keep the barrier
-// busy for about 1000 cycles.
+// One arrival for a whole warp (its lanes' writes come before it).
 __device__ __forceinline__ void warp_arrive(uint64_t* bar) {
     __syncwarp();
     if ((threadIdx.x & 31) == 0) mbar_arrive(bar);

@@ -59,7 +59,7 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t alo, uint32_t
 // 128 bytes with the 128-byte swizzle: 16-byte chunk c of token t lies at chunk
 // c ^ (t % 8).  An MMA's step is 16 tokens on.
 // In a descriptor's low word, 16 bytes count 1: the issuing thread adds offsets to
-// words made once (made anew for each MMA they took it 100 cycles apiece).
+// words made once.
 constexpr uint32_t W8_STEP = 16 * 128 / 16;
 template <int BT>
 __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
@@ -643,8 +643,7 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     if (p.slices > 1 && !p.work) return MMB_ERR_WORKSPACE;
     W8Maps maps;
     // 16-bit dy and a pair of groups as (column in a block, token, block) where their
-    // widths are whole blocks: one copy a tile instead of one a block (a copy costs the
-    // producer about 200 cycles)
+    // widths are whole blocks: one copy a tile instead of one a block
     p.dy_blocks = !D::F32 && p.N % 64 == 0;
     p.q_blocks = D::AG > 1 && p.K % W8_BK == 0;
     const bool okd =
