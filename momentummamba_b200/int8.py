@@ -67,6 +67,7 @@ def _index(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
     for t in others:
         if t is not None and t.get_device() != idx:
             idx = -1
+            break
     if idx < 0:
         _lib.require_cuda(first, *others)
     return idx
@@ -164,7 +165,7 @@ class Q8Rows:
     __slots__ = ("q", "scale")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
-        if q.dtype != torch.int8 or scale.dtype != torch.float32:
+        if q.dtype is not torch.int8 or scale.dtype is not torch.float32:
             raise ValueError(f"Q8Rows: q must be int8 and scale fp32, got {q.dtype}, {scale.dtype}")
         if q.shape[:-1] != scale.shape:
             raise ValueError(f"Q8Rows: one scale a row is wanted, got q {tuple(q.shape)} and "
@@ -263,21 +264,20 @@ def quantize_rows(x: torch.Tensor) -> Q8Rows:
     return _norm_q8(x, None, None, 0.0, 0, "quantize_rows")[0]
 
 
-def _tma_rows(t: torch.Tensor) -> torch.Tensor:
-    """int8 (rows, cols) whose rows start on 16-byte boundaries: t itself where they do."""
+def _tma_rows(t: torch.Tensor):
+    """(pointer, row stride, tensor) of int8 (rows, cols) whose rows start on 16-byte
+    boundaries: t itself where they do, else a copy."""
     rows, cols = t.shape
     s0, s1 = t.stride()
-    if (s1 == 1 or cols == 1) and t.data_ptr() % 16 == 0 and (
-            rows == 1 or (s0 % 16 == 0 and s0 >= cols)):
-        return t
+    p = t.data_ptr()
+    if (s1 == 1 or cols == 1) and not p & 15:
+        if rows == 1:  # its stride says nothing: whichever multiple of 16 holds the row
+            return p, (cols + 15) // 16 * 16, t
+        if not s0 & 15 and s0 >= cols:
+            return p, s0, t
     out = _empty_q(rows, cols, t.device)
     out.copy_(t)
-    return out
-
-
-def _ld16(t: torch.Tensor) -> int:
-    """Row stride for the tensor maps: one row has whichever multiple of 16 holds it."""
-    return t.stride(0) if t.shape[0] > 1 else (t.shape[1] + 15) // 16 * 16
+    return out.data_ptr(), out.stride(0), out
 
 
 def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
@@ -290,25 +290,33 @@ def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
     xq, wq, xs, ws = x.q, w.q, x.scale, w.scale
     idx = _index(xq, xs, wq, ws, bias)
     code = _out_type(out_dtype)
-    if wq.dim() != 2 or xq.dim() < 1 or xq.shape[-1] != wq.shape[1]:
-        raise ValueError(f"linear_q8: x (..., K) and w (N, K) must share K, got {tuple(xq.shape)} "
-                         f"and {tuple(wq.shape)}")
-    N, K = wq.shape
+    shape, wshape = xq.shape, wq.shape
+    if len(wshape) != 2 or not shape or shape[-1] != wshape[1]:
+        raise ValueError(f"linear_q8: x (..., K) and w (N, K) must share K, got {tuple(shape)} "
+                         f"and {tuple(wshape)}")
+    N, K = wshape
     if not 1 <= K <= 131071 or N < 1:
         raise ValueError(f"linear_q8: K must be 1..131071 and N at least 1, got K {K}, N {N}")
+    bp = None
     if bias is not None:
         if bias.dim() != 1 or bias.shape[0] != N:
             raise ValueError(f"linear_q8: bias must be ({N},), got {tuple(bias.shape)}")
         if bias.dtype != torch.float32 or bias.stride(0) != 1:
             bias = bias.detach().float().contiguous()
-    out = torch.empty(*xq.shape[:-1], N, dtype=out_dtype, device=xq.device)
-    if xq.dim() != 2:
+        bp = bias.data_ptr()
+    if len(shape) == 2:
+        M = shape[0]
+        out = torch.empty(M, N, dtype=out_dtype, device=xq.device)
+    else:
+        out = torch.empty(*shape[:-1], N, dtype=out_dtype, device=xq.device)
         xq = xq.reshape(-1, K)
-    M = xq.shape[0]
+        M = xq.shape[0]
     if M:
-        xq, wq, xs, ws = _tma_rows(xq), _tma_rows(wq), xs.contiguous(), ws.contiguous()
-        _call("mmb_gemm_q8", idx, M, N, K, xq.data_ptr(), _ld16(xq), xs.data_ptr(), wq.data_ptr(),
-              _ld16(wq), ws.data_ptr(), _p(bias), code, out.data_ptr(), N)
+        xp, ldx, xq = _tma_rows(xq)
+        wp, ldw, wq = _tma_rows(wq)
+        xs, ws = xs.contiguous(), ws.contiguous()
+        _call("mmb_gemm_q8", idx, M, N, K, xp, ldx, xs.data_ptr(), wp, ldw, ws.data_ptr(), bp, code,
+              out.data_ptr(), N)
     return out
 
 
@@ -472,13 +480,14 @@ def _weight_grad(idx, dy, code, q, scale_ptr, row_ptr, col_ptr, out_dtype, oc):
     M, K = q.shape
     N = dy.shape[-1]
     dw = torch.empty(N, K, dtype=out_dtype, device=dy.device)
-    dy2, q = _tma_grad(dy), _tma_rows(q)
+    dy2 = _tma_grad(dy)
+    qp, ldq, q = _tma_rows(q)
     floats = _wgrad_floats(M, N, K, code)
     work = torch.empty(floats, dtype=torch.float32, device=dy.device) if floats else None
     unit = 16 // dy.element_size()
     _call("mmb_wgrad_ck8", idx, M, N, K, code, dy2.data_ptr(),
-          dy2.stride(0) if M > 1 else -(-N // unit) * unit, q.data_ptr(), _ld16(q), scale_ptr,
-          row_ptr, col_ptr, oc, dw.data_ptr(), K, _p(work))
+          dy2.stride(0) if M > 1 else -(-N // unit) * unit, qp, ldq, scale_ptr, row_ptr, col_ptr, oc,
+          dw.data_ptr(), K, _p(work))
     return dw
 
 
