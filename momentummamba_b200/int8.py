@@ -211,7 +211,7 @@ def _made(cls, q, scale):
 def _restore(q, scale, grouped, dtype):
     idx = _index(q, scale)
     code = _out_type(dtype)
-    out = torch.empty(q.shape, dtype=dtype, device=q.device)
+    out = torch.empty(*q.shape, dtype=dtype, device=q.device)
     n = out.numel()
     if n:
         cols = q.shape[-1]
