@@ -33,7 +33,7 @@
 // Everything here is bound by HBM: each value is read once and written once.
 // B200, 65536 x 1024 bf16 (bytes at the measured 6.55 TB/s copy rate beside it):
 // 8-bit rows 72 us (72), checkpointed norm 93 (92), its backward with the column
-// sums 98 (72: blocks walk rows, and a row's load, reduction and store follow one
+// sums 90 (72: blocks walk rows, and a row's load, reduction and store follow one
 // another), restoring 33 (31).  65536 x 1001 fp16, single loads: 101 (70),
 // 136 (90), 134 (70); these are bound by the number of accesses.
 #include <cuda_bf16.h>
@@ -491,8 +491,10 @@ struct R8Bwd {
 // registers; at the end a block's rows-in-flight are added up in shared memory
 // and the block writes its own line of partial sums, which r8_colsum_kernel adds
 // in a fixed order: the result does not depend on timing.
+// Blocks of 128 threads run four an SM: 153 registers a thread left three (65536 x
+// 1024 bf16: 102 us against 94).  Single loads keep their registers, and three.
 template <class EN, class EX, bool VEC, int NC, int U, int NT, int LPR = 32>
-__global__ void __launch_bounds__(NT) r8_bwd_kernel(const R8Bwd p) {
+__global__ void __launch_bounds__(NT, VEC && NT == 128 ? 4 : 1) r8_bwd_kernel(const R8Bwd p) {
     extern __shared__ float r8_acc[];  // blockDim.y x cols, when blockDim.y > 1
     __shared__ float2 part[R8_MAX_WARPS];
     constexpr int RPW = 32 / LPR;
@@ -717,8 +719,8 @@ static int r8_fwd_launch(const R8Fwd& p, const R8Shape& s, cudaStream_t st) {
     else if (s.nc == 2 && s.warps == 1)
         r8_fwd_kernel<EX, ER, VEC, 2, 128, CK><<<grid, block, 0, st>>>(p);
     else if (s.nc == 2) r8_fwd_kernel<EX, ER, VEC, 2, 512, CK><<<grid, block, 0, st>>>(p);
-    else if (s.warps == 1) r8_fwd_kernel<EX, ER, VEC, 4, 128, CK><<<grid, block, 0, st>>>(p);
-    else r8_fwd_kernel<EX, ER, VEC, 4, 512, CK><<<grid, block, 0, st>>>(p);
+    else if (s.warps > 1) r8_fwd_kernel<EX, ER, VEC, 4, 512, CK><<<grid, block, 0, st>>>(p);
+    else if constexpr (VEC) r8_fwd_kernel<EX, ER, VEC, 4, 128, CK><<<grid, block, 0, st>>>(p);
     return mmb_launch_status();
 }
 template <class EX, class ER>
@@ -754,13 +756,19 @@ static int r8_fwd_check(const R8Fwd& p, int xt, int rt) {
     return MMB_OK;
 }
 
+// The backward's shape: fp32 gradients of three or four chunks take two warps a row
+// (65536 x 1024 fp32: 175 -> 157 us).
+static R8Shape r8_bwd_shape(int64_t cols, bool vec, bool f32) {
+    const int64_t chunks = (cols + R8_CHUNK - 1) / R8_CHUNK;
+    return r8_shape(cols, vec && !(f32 && (chunks == 3 || chunks == 4)));
+}
 // Blocks of the backward: enough to fill the GPU, few enough that the lines of
 // partial sums stay small.
-static int r8_bwd_blocks(int64_t rows, const R8Shape& s) {
+static int r8_bwd_blocks(int64_t rows, const R8Shape& s, bool vec) {
     const int64_t need = (rows + s.rows - 1) / s.rows;
-    // as many as are resident at once: a fourth block of 128 threads an SM waited for
-    // the others to end (65536 x 1024 bf16: 133 us)
-    const int64_t most = 148 * (s.rows > 1 ? 3 : s.warps < 16 ? 16 / s.warps : 1);
+    // as many as are resident at once: one more an SM waits for the others to end
+    // (65536 x 1024 bf16, four blocks where three fit: 133 us)
+    const int64_t most = 148 * (s.rows > 1 ? (vec ? 4 : 3) : s.warps < 16 ? 16 / s.warps : 1);
     return (int)min64(need, most);
 }
 template <class EN, class EX, bool VEC>
@@ -776,8 +784,9 @@ static int r8_bwd_launch(const R8Bwd& p, const R8Shape& s, int blocks, cudaStrea
     else if (s.nc == 2 && s.warps == 1)
         r8_bwd_kernel<EN, EX, VEC, 2, 2, 128><<<blocks, block, sm, st>>>(p);
     else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, VEC ? 2 : 1, 512><<<blocks, block, sm, st>>>(p);
-    else if (s.warps == 1) r8_bwd_kernel<EN, EX, VEC, 4, 1, 128><<<blocks, block, sm, st>>>(p);
-    else r8_bwd_kernel<EN, EX, VEC, 4, 1, 512><<<blocks, block, sm, st>>>(p);
+    else if (s.warps > 1) r8_bwd_kernel<EN, EX, VEC, 4, 1, 512><<<blocks, block, sm, st>>>(p);
+    else if constexpr (VEC && sizeof(typename EN::T) == 2)
+        r8_bwd_kernel<EN, EX, VEC, 4, 1, 128><<<blocks, block, sm, st>>>(p);
     return mmb_launch_status();
 }
 
@@ -819,10 +828,11 @@ extern "C" int mmb_norm_ck8_fwd(int64_t rows, int64_t cols, int32_t x_type, cons
 
 extern "C" size_t mmb_norm_ck8_bwd_work_floats(int64_t rows, int64_t cols) {
     if (rows <= 0 || cols <= 0) return 0;
-    // the loads' form is not known here: the larger of the two
+    // the loads' form is not known here: the larger of the two (every shape of the
+    // backward is one of r8_shape's)
     const R8Shape a = r8_shape(cols, false), b = r8_shape(cols, true);
     if (!a.nc) return 0;
-    const int na = r8_bwd_blocks(rows, a), nb = r8_bwd_blocks(rows, b);
+    const int na = r8_bwd_blocks(rows, a, false), nb = r8_bwd_blocks(rows, b, true);
     return (size_t)(na > nb ? na : nb) * (size_t)cols;
 }
 
@@ -850,9 +860,9 @@ extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, con
     const int nb = r8_bytes(dn_type), xb = r8_bytes(dx_type);
     const bool vec = cols % 8 == 0 && r8_aligned(dn, lddn, nb) && r8_aligned(dh, lddh, xb) &&
                      r8_aligned(dx, lddx, xb) && r8_aligned(weight, 0, 4) && r8_aligned_q(q, ldq);
-    const R8Shape s = r8_shape(cols, vec);
+    const R8Shape s = r8_bwd_shape(cols, vec, dn_type == MMB_F32);
     if (!s.nc) return MMB_ERR_UNSUPPORTED;
-    const int blocks = r8_bwd_blocks(rows, s);
+    const int blocks = r8_bwd_blocks(rows, s, vec);
     int rc;
 #define R8_BWD(EN, EX)                                                \
     (vec ? r8_bwd_launch<EN, EX, true>(p, s, blocks, st)              \
