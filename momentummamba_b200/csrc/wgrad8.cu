@@ -20,13 +20,13 @@
 //     accumulator, the two small ones into another.
 //
 // Tile: one or two groups of 128 checkpoint columns (a token has one scale in
-// each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a token's
-// values are contiguous; tokens are the reduction).  The tokens are cut into
-// slices so that tiles x slices fill the GPU; a slice's tile goes to a
-// workspace and w8_sum_kernel adds the slices in a fixed order.  Persistent,
-// one CTA per SM, roles in separate warps over one ring of token blocks:
-// producer, MMA issuer (two TMEM accumulators), converters, four epilogue
-// warps.  Every wait is bounded.
+// each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a
+// token's values are contiguous; tokens are the reduction).  The tokens are cut
+// into slices so that tiles x slices fill the GPU; a slice's tile goes to a
+// workspace and w8_sum_kernel adds the slices in a fixed order.  Persistent, one
+// CTA per SM, roles in separate warps over two rings of token blocks, one of
+// blocks as they are loaded and one of widened ones: producer (TMA), the tokens'
+// factors (cp.async), MMA issuer, converters, epilogue.  Every wait is bounded.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -69,8 +69,8 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 // AG: checkpoint groups (128 columns) of a tile; BN: its dy columns; BT: tokens of
 // a block; RL, RC: blocks in flight as they lie in memory / widened; RA:
 // accumulators; CW, EW: converter (in CG groups, each at a block of its own) and
-// epilogue warps; SEG: token blocks that
-// accumulate in TMEM before the sums move to registers.
+// epilogue warps; SEG: token blocks that accumulate in TMEM before the sums move
+// to registers.
 //
 // Two groups share each load of dy (65536 x (4096, 1024) bf16: 815 -> 560 us).
 //
