@@ -9,15 +9,15 @@
 // the norm's output has to be kept.
 //
 // The kept values are never written out: each CTA loads the bytes, widens them
-// in shared memory and multiplies.
-//   * 16-bit dy goes from TMA to the tensor cores as it is; the kept values are
-//     widened to its type.  q * s is exact there (7 bits and a power of two, in
-//     bf16 for any s, in fp16 within its range); with `row` the product
-//     q * s * row is rounded to that type, half a unit of 2^-8 (bf16) or 2^-11
-//     (fp16), below the half step that q itself is off by.
-//   * fp32 dy (times row, in fp32) is split into three bf16 parts, 24 bits in
-//     all, and multiplied with the exact q * s: the high part into one
-//     accumulator, the two small ones into another.
+// in shared memory and multiplies.  q * s has 7 bits and a power of two, so it is
+// exact in the 16 bits it is multiplied in; `row` goes to the other operand.
+//   * 16-bit dy without `row` goes from TMA to the tensor cores as it is, with
+//     the kept values widened to its type (bf16 for any s, fp16 within its range).
+//   * otherwise dy (times row, in fp32) is split into bf16 parts and multiplied
+//     with q * s in bf16: 16-bit dy into two (16 bits, off by at most 2^-17 of a
+//     term; one part would be off by 2^-9, as much as a bf16 result's own
+//     rounding), fp32 dy into three (24 bits), the high part into one accumulator
+//     and the two small ones into another.
 //
 // Tile: one or two groups of 128 checkpoint columns (a token has one scale in
 // each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a
@@ -34,7 +34,7 @@
 
 namespace mmb {
 
-constexpr int W8_BK = 128;  // checkpoint columns of a tile
+constexpr int W8_BK = 128;  // checkpoint columns of a group
 constexpr uint32_t W8_SWZ128 = 2;
 
 // MMA of 16-bit operands, both MN-major, fp32 accumulation: M = 128, N = n
@@ -84,6 +84,7 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 template <bool BF, int GROUPS>
 struct W8Half {
     static constexpr bool BF16 = BF, F32 = false;
+    static constexpr int PARTS = 1;  // dy as it is
     static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2, SEG = 1 << 30;
     static constexpr int RL = AG == 1 ? 4 : 3, RC = AG == 1 ? 3 : 2, RA = AG == 1 ? 2 : 1;
     static constexpr int CW = 8, CG = 1, EW = 8;
@@ -103,10 +104,31 @@ struct W8Half {
 // the result as near as an fp32 product's.
 struct W8F32 {
     static constexpr bool BF16 = true, F32 = true;
+    static constexpr int PARTS = 3;
     static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4, SEG = 32;
     static constexpr int RL = 4, RC = 4, RA = 2, CW = 8, CG = 4, EW = 8;
     static __device__ __forceinline__ uint32_t pack2(float a, float b) {
         return W8Half<true, 1>::pack2(a, b);
+    }
+};
+// 16-bit dy (bf16 or fp16 in memory: BF) in two bf16 parts.  Blocks of 32 tokens
+// leave room for both parts of 256 columns.  Twice the MMAs of W8Half, and dy goes
+// through the converters: 65536 x (4096, 1024) bf16 880 us (one part 475), 76800 x
+// (1024, 256) 85 us (65).
+template <bool BF, int GROUPS>
+struct W8Two {
+    static constexpr bool BF16 = true, F32 = false, DY_BF16 = BF;
+    static constexpr int PARTS = 2;
+    static constexpr int AG = GROUPS, BN = 256, BT = 32, BYTES = 2, SEG = 1 << 30;
+    static constexpr int RL = 3, RC = AG == 1 ? 4 : 3, RA = AG == 1 ? 2 : 1;
+    static constexpr int CW = 8, CG = 2, EW = 8;
+    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
+        return W8Half<true, 1>::pack2(a, b);
+    }
+    // two values of dy in fp32
+    static __device__ __forceinline__ float2 dy2(uint32_t w) {
+        if constexpr (BF) return make_float2(bf16_lo(w), bf16_hi(w));
+        else return __half22float2(*reinterpret_cast<const __half2*>(&w));
     }
 };
 template <class D>
@@ -118,8 +140,8 @@ struct W8Smem {
     static constexpr int LOAD = DY + Q + FACT;
     static constexpr int A1 = D::BT * W8_BK * 2;         // widened checkpoint, one group
     static constexpr int A = D::AG * A1;
-    static constexpr int DY3 = D::F32 ? 3 * D::BT * D::BN * 2 : 0;  // dy's bf16 parts
-    static constexpr int CONV = A + DY3;
+    static constexpr int P1 = D::BT * D::BN * 2;          // one of dy's bf16 parts
+    static constexpr int CONV = A + (D::PARTS > 1 ? D::PARTS * P1 : 0);
     static constexpr size_t BYTES = (size_t)D::RL * LOAD + (size_t)D::RC * CONV + 1024;
 };
 template <class D>
@@ -159,8 +181,8 @@ __device__ __forceinline__ void w8_store(void* dw, int64_t at, int out_type, flo
 
 // 4 bytes q -> 4 floats q * f.  A byte with its sign bit flipped, q + 128, becomes
 // the second byte of the mantissa of 2^15; one fused step then takes 2^15 + 128
-// away and multiplies: (2^15 + 128 + q) * f - (2^15 + 128) * f.  With f held to 15
-// significant bits (w8_factor) both products' difference is exact.
+// away and multiplies: (2^15 + 128 + q) * f - (2^15 + 128) * f, exact for a power
+// of two.
 __device__ __forceinline__ void w8_widen4(uint32_t w, float f, float fc, float2& v0, float2& v1) {
     const uint32_t u = w ^ 0x80808080u;
     v0 = ffma2(make_float2(__uint_as_float(__byte_perm(u, 0x47000000u, 0x7404)),
@@ -169,12 +191,6 @@ __device__ __forceinline__ void w8_widen4(uint32_t w, float f, float fc, float2&
                            __uint_as_float(__byte_perm(u, 0x47000000u, 0x7434))), f2(f), f2(fc));
 }
 constexpr float W8_HUGE = 0x1p111f;
-// f rounded to 15 significant bits: exact for a power of two; with a row factor
-// 2^-16 of the value, far below the rounding to 16 bits that follows.
-__device__ __forceinline__ float w8_factor(float f) {
-    const uint32_t u = __float_as_uint(f);
-    return (u & 0x7f800000u) == 0x7f800000u ? f : __uint_as_float((u + 0x100u) & ~0x1ffu);
-}
 
 template <class D>
 __global__ void __launch_bounds__(w8_threads<D>(), 1)
@@ -218,7 +234,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
         abort_s = 0;
         for (int s = 0; s < RL; ++s) {
             mbar_init(&full[s], 1 + 32);               // TMA, and the factors of each lane
-            mbar_init(&free_l[s], D::F32 ? CGW : 1);  // read by the converters / by the MMAs
+            mbar_init(&free_l[s], D::PARTS > 1 ? CGW : 1);  // read by the converters / the MMAs
         }
         for (int c = 0; c < RC; ++c) {
             mbar_init(&conv[c], CGW);
@@ -254,7 +270,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     ok = ws_wait(&free_l[r.s], r.ph ^ 1u, abort, p.err);
                     if (!ok) break;
                     mbar_expect_tx(bar, Sm::DY + Sm::Q);
-                    if constexpr (D::F32) {
+                    if constexpr (D::PARTS > 1) {
                         tma_load_3d(slot_dy(r.s), &maps.dy, nx, m0, 0, bar);
                     } else if (p.dy_blocks) {
                         tma_load_3d(slot_dy(r.s), &maps.dy, 0, m0, ng, bar);
@@ -334,7 +350,8 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     if (!ok) break;
                     tc_fence_after();
                     const uint32_t la = lo0 + (RL * Sm::LOAD + c * Sm::CONV) / 16;
-                    const uint32_t lb = D::F32 ? la + Sm::A / 16 : lo0 + s * (Sm::LOAD / 16);
+                    const uint32_t lb =
+                        D::PARTS > 1 ? la + Sm::A / 16 : lo0 + s * (Sm::LOAD / 16);
                     const uint32_t first = in_seg > 0 ? 1u : 0u;
                     if constexpr (D::F32) {
                         // high and middle parts lie side by side: one MMA of twice the
@@ -344,17 +361,20 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                             umma_f16(acc, la + kk * W8_STEP, lb + kk * W8_STEP, dhi,
                                      w8_idesc(2 * BN, true), kk > 0 ? 1u : first);
                             umma_f16(acc + BN, la + kk * W8_STEP,
-                                     lb + 2 * (BT * BN * 2 / 16) + kk * W8_STEP, dhi, IDESC, 1u);
+                                     lb + 2 * (Sm::P1 / 16) + kk * W8_STEP, dhi, IDESC, 1u);
                         }
                     } else {
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk)
 #pragma unroll
-                            for (int g = 0; g < AG; ++g)
-                                umma_f16(acc + g * BN, la + g * (Sm::A1 / 16) + kk * W8_STEP,
-                                         lb + kk * W8_STEP, dhi, IDESC, kk > 0 ? 1u : first);
+                            for (int i = 0; i < D::PARTS; ++i)
+#pragma unroll
+                                for (int g = 0; g < AG; ++g)
+                                    umma_f16(acc + g * BN, la + g * (Sm::A1 / 16) + kk * W8_STEP,
+                                             lb + i * (Sm::P1 / 16) + kk * W8_STEP, dhi, IDESC,
+                                             kk > 0 || i > 0 ? 1u : first);
                     }
-                    if constexpr (!D::F32) umma_commit(&free_l[s]);
+                    if constexpr (D::PARTS == 1) umma_commit(&free_l[s]);
                     umma_commit(&free_c[c]);
                     if (in_seg == D::SEG - 1 || b == nb - 1) {
                         umma_commit(&acc_full[a]);
@@ -401,14 +421,13 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     const int g = gi / PIECES, t = t0 + gi % PIECES * (CT / 8);
                     w[gi] = lds16(qs + g * Sm::Q1 + t * W8_BK);
                     fa[gi] = lds4f(fs + 4 * (g * BT + t));
-                    if (!D::F32 && p.row) fa[gi] *= lds4f(fs + 4 * (ROW + t));
                     huge |= fabsf(fa[gi]) >= W8_HUGE;
                 }
                 const auto widen = [&](float shrink, float grow) {
 #pragma unroll
                     for (int gi = 0; gi < AG * PIECES; ++gi) {
                         const int g = gi / PIECES, t = t0 + gi % PIECES * (CT / 8);
-                        const float f = w8_factor(fa[gi] * shrink), fc = -32896.f * f;
+                        const float f = fa[gi] * shrink, fc = -32896.f * f;
                         const uint32_t ws[4] = {w[gi].x, w[gi].y, w[gi].z, w[gi].w};
                         uint32_t o[8];
 #pragma unroll
@@ -458,7 +477,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 #pragma unroll
                             for (int part = 0; part < 3; ++part) {
                                 const uint32_t o0 = D::pack2(v0.x, v0.y), o1 = D::pack2(v1.x, v1.y);
-                                sts8(dst + part * (BT * BN * 2), o0, o1);
+                                sts8(dst + part * Sm::P1, o0, o1);
                                 v0.x -= bf16_lo(o0);
                                 v0.y -= bf16_hi(o0);
                                 v1.x -= bf16_lo(o1);
@@ -467,9 +486,45 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                         }
                     }
                 }
+                if constexpr (D::PARTS == 2) {
+                    // dy * row = high + low, each bf16: 8 neighbouring lanes take the 128
+                    // bytes of a block of 64 columns of one token
+                    const int c = ct & 7;
+                    constexpr int ITEMS = BT * (BN / 64), STEPS = ITEMS / (CT / 8), AT_ONCE = 4;
+                    static_assert(STEPS % AT_ONCE == 0, "whole batches");
+                    const uint32_t ds = smem_u32(slot_dy(s)) + c * 16;
+#pragma unroll
+                    for (int i0 = 0; i0 < STEPS; i0 += AT_ONCE) {
+                        uint4 x[AT_ONCE];
+                        float r[AT_ONCE];
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i) {
+                            const int item = (ct >> 3) + (i0 + i) * (CT / 8);
+                            const int t = item / (BN / 64), h = item % (BN / 64);
+                            x[i] = lds16(ds + t * (BN * 2) + h * 128);
+                            r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i) {
+                            const int item = (ct >> 3) + (i0 + i) * (CT / 8);
+                            const int t = item / (BN / 64), h = item % (BN / 64);
+                            const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float2 v = fmul2(D::dy2(xs[e]), f2(r[i]));
+                                hi[e] = D::pack2(v.x, v.y);
+                                lo[e] = D::pack2(v.x - bf16_lo(hi[e]), v.y - bf16_hi(hi[e]));
+                            }
+                            const uint32_t dst = as + Sm::A + w8_chunk<BT>(h, t, c);
+                            sts16(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+                            sts16(dst + Sm::P1, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                        }
+                    }
+                }
                 fence_proxy_async_smem();
                 warp_arrive(&conv[cs]);
-                if constexpr (D::F32) warp_arrive(&free_l[s]);
+                if constexpr (D::PARTS > 1) warp_arrive(&free_l[s]);
             }
         }
     } else {
@@ -610,7 +665,7 @@ template <class D>
 static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t nblk = (M + D::BT - 1) / D::BT, kt = D::AG * W8_BK;
     const int64_t tiles = (K + kt - 1) / kt * ((N + D::BN - 1) / D::BN);
-    const double block_us = D::F32 ? 0.25 : D::AG == 1 ? 0.45 : 0.60;
+    const double block_us = D::F32 ? 0.25 : D::AG == 1 ? 0.45 : 0.60;  // a block of BT tokens
     const double tile_us = 1.0 + D::AG * (D::F32 ? 0.5 : 1.0);
     const double slice_us = 2.0 * (double)N * (double)K * 4.0 / 5e6;
     W8Plan best{1, nblk, 1e30};
@@ -628,8 +683,14 @@ static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
     return best;
 }
 // 16-bit dy: one group a tile or two, whichever is estimated faster
+template <template <bool, int> class D>
 static bool w8_two_groups(int64_t M, int64_t N, int64_t K) {
-    return w8_plan<W8Half<true, 2>>(M, N, K).us < w8_plan<W8Half<true, 1>>(M, N, K).us;
+    return w8_plan<D<true, 2>>(M, N, K).us < w8_plan<D<true, 1>>(M, N, K).us;
+}
+template <template <bool, int> class D>
+static int64_t w8_slices(int64_t M, int64_t N, int64_t K) {
+    return w8_two_groups<D>(M, N, K) ? w8_plan<D<true, 2>>(M, N, K).slices
+                                     : w8_plan<D<true, 1>>(M, N, K).slices;
 }
 static int64_t w8_pitch(int64_t K) { return (K + 3) / 4 * 4; }
 
@@ -642,12 +703,13 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     p.ldp = w8_pitch(p.K);
     if (p.slices > 1 && !p.work) return MMB_ERR_WORKSPACE;
     W8Maps maps;
-    // 16-bit dy and a pair of groups as (column in a block, token, block) where their
-    // widths are whole blocks: one copy a tile instead of one a block
-    p.dy_blocks = !D::F32 && p.N % 64 == 0;
+    // dy that is multiplied as it is and a pair of groups as (column in a block, token,
+    // block) where their widths are whole blocks: one copy a tile instead of one a block
+    p.dy_blocks = D::PARTS == 1 && p.N % 64 == 0;
     p.q_blocks = D::AG > 1 && p.K % W8_BK == 0;
     const bool okd =
-        D::F32 ? mmb_encode_tile_map(&maps.dy, dy, 4, p.N, p.M, 1, lddy, lddy * p.M, D::BN, D::BT, 0)
+        D::PARTS > 1 ? mmb_encode_tile_map(&maps.dy, dy, D::BYTES, p.N, p.M, 1, lddy, lddy * p.M,
+                                           D::BN, D::BT, 0)
         : p.dy_blocks
             ? mmb_encode_tile_map(&maps.dy, dy, 2, 64, p.M, p.N / 64, lddy, 64, 64, D::BT, 128,
                                   D::BN / 64)
@@ -673,16 +735,32 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     return mmb_launch_status();
 }
 
+template <template <bool, int> class D>
+static int w8_launch16(const W8Params& p, int dy_type, const void* dy, int64_t lddy,
+                       const int8_t* q, int64_t ldq, cudaStream_t s) {
+    const bool two = w8_two_groups<D>(p.M, p.N, p.K);
+    if (dy_type == MMB_BF16)
+        return two ? w8_launch<D<true, 2>>(p, dy, lddy, q, ldq, s)
+                   : w8_launch<D<true, 1>>(p, dy, lddy, q, ldq, s);
+    return two ? w8_launch<D<false, 2>>(p, dy, lddy, q, ldq, s)
+               : w8_launch<D<false, 1>>(p, dy, lddy, q, ldq, s);
+}
+
 }  // namespace mmb
 
 using namespace mmb;
 
 extern "C" size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int32_t dy_type) {
     if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
-    const W8Plan plan = dy_type == MMB_F32        ? w8_plan<W8F32>(M, N, K)
-                        : w8_two_groups(M, N, K) ? w8_plan<W8Half<true, 2>>(M, N, K)
-                                                 : w8_plan<W8Half<true, 1>>(M, N, K);
-    return plan.slices > 1 ? (size_t)plan.slices * (size_t)N * (size_t)w8_pitch(K) : 0;
+    // whether there is a row factor is not known here: the larger of the two forms
+    int64_t slices;
+    if (dy_type == MMB_F32) {
+        slices = w8_plan<W8F32>(M, N, K).slices;
+    } else {
+        const int64_t a = w8_slices<W8Half>(M, N, K), b = w8_slices<W8Two>(M, N, K);
+        slices = a > b ? a : b;
+    }
+    return slices > 1 ? (size_t)slices * (size_t)N * (size_t)w8_pitch(K) : 0;
 }
 
 extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, const void* dy,
@@ -716,10 +794,6 @@ extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, c
     p.dw = dw; p.ldw = ldw; p.out_type = out_type; p.work = work;
     p.err = mmb_device_error_flag();
     if (dy_type == MMB_F32) return w8_launch<W8F32>(p, dy, lddy, q, ldq, s);
-    const bool two = w8_two_groups(M, N, K);
-    if (dy_type == MMB_BF16)
-        return two ? w8_launch<W8Half<true, 2>>(p, dy, lddy, q, ldq, s)
-                   : w8_launch<W8Half<true, 1>>(p, dy, lddy, q, ldq, s);
-    return two ? w8_launch<W8Half<false, 2>>(p, dy, lddy, q, ldq, s)
-               : w8_launch<W8Half<false, 1>>(p, dy, lddy, q, ldq, s);
+    return row ? w8_launch16<W8Two>(p, dy_type, dy, lddy, q, ldq, s)
+               : w8_launch16<W8Half>(p, dy_type, dy, lddy, q, ldq, s);
 }

@@ -1,0 +1,82 @@
+"""weight_grad_ckpt where 16 bits do not hold an operand: behind a norm, dy times the
+row's factor has more bits than its type and is multiplied in two bf16 parts.
+
+Tolerance, for S = sum of |terms|: dy * row is rounded once in fp32 (2^-24); the high
+part leaves at most 2^-9 of it and the low part 2^-9 of that (2^-18); the tensor cores
+add 16 terms a step, each step off by at most 2^-23 of a partial sum, two steps for 16
+tokens, and slices of the tokens one step each (148 at most).  Rounded to 16 bits
+between (2^-9 or 2^-12 a term), a result of a few tokens is far outside.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DEV = "cuda:0"
+
+
+def make(M, N, K, x_type, dy_type, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed * 65537 + M * 131 + N * 17 + K)
+    x = (torch.randn(M, K, generator=g, device=DEV) * torch.exp(torch.randn(K, generator=g, device=DEV))).to(x_type)
+    dy = torch.randn(M, N, generator=g, device=DEV).to(dy_type)
+    row = torch.rand(M, generator=g, device=DEV) + 0.5
+    col = 1 + 0.2 * torch.randn(K, generator=g, device=DEV)
+    return x, dy, row, col
+
+
+def products64(dy, kept, row, col):
+    """(the gradient, the sum of its terms' sizes) in 64 bits."""
+    a = dy.double() if row is None else dy.double() * row.double()[:, None]
+    want, size = a.t() @ kept.double(), a.abs().t() @ kept.double().abs()
+    return (want, size) if col is None else (want * col.double(), size * col.double().abs())
+
+
+def two_parts(M):
+    return (2 * -(-M // 16) + 150) * 2.0 ** -23 + 2.0 ** -18 + 2 * 2.0 ** -24
+
+
+# one group and two groups a tile, one slice and several, whole and partial blocks
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (5, 24, 40), (33, 257, 129), (100, 700, 333), (64, 4096, 1024),
+                                   (500, 200, 300), (700, 1032, 2000)], ids=lambda v: str(v))
+def test_behind_a_norm_with_an_fp32_result(M, N, K, dtype):
+    from momentummamba_b200 import int8
+    x, dy, row, col = make(M, N, K, dtype, dtype)
+    ck = int8.checkpoint_rows(x)
+    dw = int8.weight_grad_ckpt(dy, ck, row, col, out_dtype=torch.float32)
+    want, size = products64(dy, ck.restore(), row, col)
+    assert torch.all((dw.double() - want).abs() <= two_parts(M) * size + 2.0 ** -23 * want.abs())
+    assert torch.equal(dw, int8.weight_grad_ckpt(dy, ck, row, col, out_dtype=torch.float32))
+
+
+def test_a_16_bit_result_is_rounded_once():
+    """Over many tokens the result stands as near to 64 bits as rounding alone allows: a
+    uniform error of half a unit in the last place, 2^-8 / (2 sqrt(3)) = 1.13e-3 of values
+    at the low end of a binade and half of that at the high end, 0.82e-3..1.7e-3 over a
+    normal distribution; an operand rounded to bf16 as well adds 1.6e-3 in square."""
+    from momentummamba_b200 import int8
+    x, dy, row, col = make(8192, 512, 256, torch.bfloat16, torch.bfloat16)
+    ck = int8.checkpoint_rows(x)
+    dw = int8.weight_grad_ckpt(dy, ck, row, col)
+    want, _ = products64(dy, ck.restore(), row, col)
+    ideal = float((want.bfloat16().double() - want).norm())
+    assert dw.dtype == torch.bfloat16
+    assert float((dw.double() - want).norm()) <= 1.01 * ideal
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+def test_fp32_weights_under_autocast(dtype):
+    """norm_linear_ckpt's own weight gradient: fp32 weights, a 16-bit product."""
+    from momentummamba_b200 import int8
+    M, N, K = 300, 64, 200
+    x, dy, _, col = make(M, N, K, torch.float32, dtype)
+    W = torch.randn(N, K, device=DEV, requires_grad=True)
+    with torch.autocast("cuda", dtype=dtype):
+        y, _ = int8.norm_linear_ckpt(x, col, W)
+    assert y.dtype == dtype
+    (dw,) = torch.autograd.grad(y, W, dy)
+    rstd = 1 / torch.sqrt((x.double() ** 2).mean(1) + 1e-5)
+    want, size = products64(dy, int8.checkpoint_rows(x).restore(), rstd, col)
+    # the kernel's own rstd is off by 4e-6 at most
+    assert dw.dtype == torch.float32
+    assert torch.all((dw.double() - want).abs() <= (two_parts(M) + 4e-6) * size + 2.0 ** -23 * want.abs())
