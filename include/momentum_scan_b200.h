@@ -543,10 +543,10 @@ int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, c
  * fp32 accumulation):
  *   dw[n, k] = col[k] * sum_m dy[m, n] * row[m] * q[m, k] * s[m, k / 128]
  * dy (M, N) of dy_type; q (M, K), scale (M, ceil(K / 128)) as mmb_norm_ck8_fwd
- * keeps them; row (M) and col (K) nullable: a norm's rstd and weight.  16-bit dy
- * without row is multiplied as it is with the kept values in its type (fp16: kept
- * values beyond its range become infinities); 16-bit dy * row in two bf16 parts
- * (16 bits), fp32 dy (* row) in three (24 bits).
+ * keeps them; row (M) and col (K) nullable: a norm's rstd and weight.  The kept
+ * values are multiplied in bf16, where they are exact; bf16 dy without row as it
+ * is, other 16-bit dy (* row) in two bf16 parts (16 bits), fp32 dy (* row) in three
+ * (24 bits).
  * dw (N, K) of out_type.  M == 0 clears dw.  dy and q 16-byte aligned, lddy a
  * multiple of 16 bytes, ldq of 16.  work (16-byte aligned) holds
  * mmb_wgrad_ck8_work_floats floats; results repeat bit for bit. */

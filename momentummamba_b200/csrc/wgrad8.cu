@@ -10,14 +10,14 @@
 //
 // The kept values are never written out: each CTA loads the bytes, widens them
 // in shared memory and multiplies.  q * s has 7 bits and a power of two, so it is
-// exact in the 16 bits it is multiplied in; `row` goes to the other operand.
-//   * 16-bit dy without `row` goes from TMA to the tensor cores as it is, with
-//     the kept values widened to its type (bf16 for any s, fp16 within its range).
-//   * otherwise dy (times row, in fp32) is split into bf16 parts and multiplied
-//     with q * s in bf16: 16-bit dy into two (16 bits, off by at most 2^-17 of a
-//     term; one part would be off by 2^-9, as much as a bf16 result's own
-//     rounding), fp32 dy into three (24 bits), the high part into one accumulator
-//     and the two small ones into another.
+// exact in bf16, whatever s; `row` goes to the other operand.
+//   * bf16 dy without `row` goes from TMA to the tensor cores as it is.
+//   * otherwise dy (times row, in fp32) is split into bf16 parts: 16-bit dy into
+//     two (16 bits: exact without row, with it off by at most 2^-17 of a term; one
+//     part would be off by 2^-9, as much as a bf16 result's own rounding), fp32 dy
+//     into three (24 bits), the high part into one accumulator and the two small
+//     ones into another.  fp16 dy is not multiplied as it is, since fp16 does not
+//     hold what a checkpoint may: kept values reach from 2^-100 to fp32's largest.
 //
 // Tile: one or two groups of 128 checkpoint columns (a token has one scale in
 // each) as the MMA's rows, BN columns of dy as its columns, both "MN-major" (a
@@ -37,10 +37,10 @@ namespace mmb {
 constexpr int W8_BK = 128;  // checkpoint columns of a group
 constexpr uint32_t W8_SWZ128 = 2;
 
-// MMA of 16-bit operands, both MN-major, fp32 accumulation: M = 128, N = n
-__host__ __device__ constexpr uint32_t w8_idesc(int n, bool bf16) {
-    return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | (1u << 15) |
-           (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+// MMA of bf16 operands, both MN-major, fp32 accumulation: M = 128, N = n
+__host__ __device__ constexpr uint32_t w8_idesc(int n) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) |
+           ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
 }
 // alo, blo: the low words of the operands' descriptors; they share the high one
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint32_t alo, uint32_t blo, uint32_t dhi,
@@ -81,35 +81,23 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 // 0.72 of the measured bf16 rate (400 us with the converters left out); 76800 x
 // (1024, 256) bf16 60 us.  fp32, three parts: 76800 x (1024, 256) 158 us, 32768 x
 // (512, 128) 29 us.
-template <bool BF, int GROUPS>
+template <int GROUPS>
 struct W8Half {
-    static constexpr bool BF16 = BF, F32 = false;
+    static constexpr bool F32 = false;
     static constexpr int PARTS = 1;  // dy as it is
     static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2, SEG = 1 << 30;
     static constexpr int RL = AG == 1 ? 4 : 3, RC = AG == 1 ? 3 : 2, RA = AG == 1 ? 2 : 1;
     static constexpr int CW = 8, CG = 1, EW = 8;
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        if constexpr (BF) {
-            const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
-            return *reinterpret_cast<const uint32_t*>(&t);
-        } else {
-            const __half2 t = __floats2half2_rn(a, b);
-            return *reinterpret_cast<const uint32_t*>(&t);
-        }
-    }
 };
 // The tensor cores' fp32 accumulation truncates: its error grows with the number
 // of steps.  1024 tokens (64 steps) at a time, added to sums in registers with
 // ordinary rounding, and the small parts in an accumulator of their own, keep
 // the result as near as an fp32 product's.
 struct W8F32 {
-    static constexpr bool BF16 = true, F32 = true;
+    static constexpr bool F32 = true;
     static constexpr int PARTS = 3;
     static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4, SEG = 32;
     static constexpr int RL = 4, RC = 4, RA = 2, CW = 8, CG = 4, EW = 8;
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        return W8Half<true, 1>::pack2(a, b);
-    }
 };
 // 16-bit dy (bf16 or fp16 in memory: BF) in two bf16 parts.  Blocks of 32 tokens
 // leave room for both parts of 256 columns.  Twice the MMAs of W8Half, and dy goes
@@ -117,14 +105,11 @@ struct W8F32 {
 // (1024, 256) 85 us (65).
 template <bool BF, int GROUPS>
 struct W8Two {
-    static constexpr bool BF16 = true, F32 = false, DY_BF16 = BF;
+    static constexpr bool F32 = false;
     static constexpr int PARTS = 2;
     static constexpr int AG = GROUPS, BN = 256, BT = 32, BYTES = 2, SEG = 1 << 30;
     static constexpr int RL = 3, RC = AG == 1 ? 4 : 3, RA = AG == 1 ? 2 : 1;
     static constexpr int CW = 8, CG = 2, EW = 8;
-    static __device__ __forceinline__ uint32_t pack2(float a, float b) {
-        return W8Half<true, 1>::pack2(a, b);
-    }
     // two values of dy in fp32
     static __device__ __forceinline__ float2 dy2(uint32_t w) {
         if constexpr (BF) return make_float2(bf16_lo(w), bf16_hi(w));
@@ -147,6 +132,10 @@ struct W8Smem {
 template <class D>
 __host__ __device__ constexpr int w8_threads() { return 32 * (3 + D::CW + D::EW); }
 
+__device__ __forceinline__ uint32_t w8_pack2(float a, float b) {
+    const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&t);
+}
 // `bar` counts an arrival of this lane once its cp.async copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
@@ -201,7 +190,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
     constexpr int ACC = D::F32 ? 2 * BN : AG * BN;  // TMEM columns of an accumulator
     constexpr int ROW = AG * BT;                     // place of the row factors behind the scales
     constexpr int CGW = D::CW / D::CG, CT = 32 * CGW;  // a converter group
-    constexpr uint32_t IDESC = w8_idesc(BN, D::BF16);
+    constexpr uint32_t IDESC = w8_idesc(BN);
     extern __shared__ float4 w8_smem4[];
     __shared__ uint64_t full[RL], free_l[RL], conv[RC], free_c[RC], acc_full[RA], acc_empty[RA],
         drained;
@@ -359,7 +348,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 #pragma unroll
                         for (int kk = 0; kk < BT / 16; ++kk) {
                             umma_f16(acc, la + kk * W8_STEP, lb + kk * W8_STEP, dhi,
-                                     w8_idesc(2 * BN, true), kk > 0 ? 1u : first);
+                                     w8_idesc(2 * BN), kk > 0 ? 1u : first);
                             umma_f16(acc + BN, la + kk * W8_STEP,
                                      lb + 2 * (Sm::P1 / 16) + kk * W8_STEP, dhi, IDESC, 1u);
                         }
@@ -434,8 +423,8 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                         for (int h = 0; h < 4; ++h) {
                             float2 v0, v1;
                             w8_widen4(ws[h], f, fc, v0, v1);
-                            o[2 * h] = D::pack2(v0.x * grow, v0.y * grow);
-                            o[2 * h + 1] = D::pack2(v1.x * grow, v1.y * grow);
+                            o[2 * h] = w8_pack2(v0.x * grow, v0.y * grow);
+                            o[2 * h + 1] = w8_pack2(v1.x * grow, v1.y * grow);
                         }
                         const uint32_t a = as + g * Sm::A1;
                         sts16(a + w8_chunk<BT>(blk, t, c0), make_uint4(o[0], o[1], o[2], o[3]));
@@ -476,7 +465,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                             v1 = fmul2(v1, f2(r[i]));
 #pragma unroll
                             for (int part = 0; part < 3; ++part) {
-                                const uint32_t o0 = D::pack2(v0.x, v0.y), o1 = D::pack2(v1.x, v1.y);
+                                const uint32_t o0 = w8_pack2(v0.x, v0.y), o1 = w8_pack2(v1.x, v1.y);
                                 sts8(dst + part * Sm::P1, o0, o1);
                                 v0.x -= bf16_lo(o0);
                                 v0.y -= bf16_hi(o0);
@@ -513,8 +502,8 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
                                 const float2 v = fmul2(D::dy2(xs[e]), f2(r[i]));
-                                hi[e] = D::pack2(v.x, v.y);
-                                lo[e] = D::pack2(v.x - bf16_lo(hi[e]), v.y - bf16_hi(hi[e]));
+                                hi[e] = w8_pack2(v.x, v.y);
+                                lo[e] = w8_pack2(v.x - bf16_lo(hi[e]), v.y - bf16_hi(hi[e]));
                             }
                             const uint32_t dst = as + Sm::A + w8_chunk<BT>(h, t, c);
                             sts16(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
@@ -683,14 +672,14 @@ static W8Plan w8_plan(int64_t M, int64_t N, int64_t K) {
     return best;
 }
 // 16-bit dy: one group a tile or two, whichever is estimated faster
-template <template <bool, int> class D>
+template <class One, class Two>
 static bool w8_two_groups(int64_t M, int64_t N, int64_t K) {
-    return w8_plan<D<true, 2>>(M, N, K).us < w8_plan<D<true, 1>>(M, N, K).us;
+    return w8_plan<Two>(M, N, K).us < w8_plan<One>(M, N, K).us;
 }
-template <template <bool, int> class D>
+template <class One, class Two>
 static int64_t w8_slices(int64_t M, int64_t N, int64_t K) {
-    return w8_two_groups<D>(M, N, K) ? w8_plan<D<true, 2>>(M, N, K).slices
-                                     : w8_plan<D<true, 1>>(M, N, K).slices;
+    return w8_two_groups<One, Two>(M, N, K) ? w8_plan<Two>(M, N, K).slices
+                                            : w8_plan<One>(M, N, K).slices;
 }
 static int64_t w8_pitch(int64_t K) { return (K + 3) / 4 * 4; }
 
@@ -735,15 +724,11 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     return mmb_launch_status();
 }
 
-template <template <bool, int> class D>
-static int w8_launch16(const W8Params& p, int dy_type, const void* dy, int64_t lddy,
-                       const int8_t* q, int64_t ldq, cudaStream_t s) {
-    const bool two = w8_two_groups<D>(p.M, p.N, p.K);
-    if (dy_type == MMB_BF16)
-        return two ? w8_launch<D<true, 2>>(p, dy, lddy, q, ldq, s)
-                   : w8_launch<D<true, 1>>(p, dy, lddy, q, ldq, s);
-    return two ? w8_launch<D<false, 2>>(p, dy, lddy, q, ldq, s)
-               : w8_launch<D<false, 1>>(p, dy, lddy, q, ldq, s);
+template <class One, class Two>
+static int w8_launch16(const W8Params& p, const void* dy, int64_t lddy, const int8_t* q,
+                       int64_t ldq, cudaStream_t s) {
+    return w8_two_groups<One, Two>(p.M, p.N, p.K) ? w8_launch<Two>(p, dy, lddy, q, ldq, s)
+                                                  : w8_launch<One>(p, dy, lddy, q, ldq, s);
 }
 
 }  // namespace mmb
@@ -752,13 +737,17 @@ using namespace mmb;
 
 extern "C" size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int32_t dy_type) {
     if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
-    // whether there is a row factor is not known here: the larger of the two forms
     int64_t slices;
     if (dy_type == MMB_F32) {
         slices = w8_plan<W8F32>(M, N, K).slices;
     } else {
-        const int64_t a = w8_slices<W8Half>(M, N, K), b = w8_slices<W8Two>(M, N, K);
-        slices = a > b ? a : b;
+        // bf16 and fp16 in two parts share a plan; bf16 without a row factor has its own,
+        // and whether there is one is not known here
+        slices = w8_slices<W8Two<true, 1>, W8Two<true, 2>>(M, N, K);
+        if (dy_type == MMB_BF16) {
+            const int64_t one = w8_slices<W8Half<1>, W8Half<2>>(M, N, K);
+            slices = slices > one ? slices : one;
+        }
     }
     return slices > 1 ? (size_t)slices * (size_t)N * (size_t)w8_pitch(K) : 0;
 }
@@ -794,6 +783,8 @@ extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, c
     p.dw = dw; p.ldw = ldw; p.out_type = out_type; p.work = work;
     p.err = mmb_device_error_flag();
     if (dy_type == MMB_F32) return w8_launch<W8F32>(p, dy, lddy, q, ldq, s);
-    return row ? w8_launch16<W8Two>(p, dy_type, dy, lddy, q, ldq, s)
-               : w8_launch16<W8Half>(p, dy_type, dy, lddy, q, ldq, s);
+    if (dy_type == MMB_F16)
+        return w8_launch16<W8Two<false, 1>, W8Two<false, 2>>(p, dy, lddy, q, ldq, s);
+    return row ? w8_launch16<W8Two<true, 1>, W8Two<true, 2>>(p, dy, lddy, q, ldq, s)
+               : w8_launch16<W8Half<1>, W8Half<2>>(p, dy, lddy, q, ldq, s);
 }

@@ -1,5 +1,6 @@
 """weight_grad_ckpt where 16 bits do not hold an operand: behind a norm, dy times the
-row's factor has more bits than its type and is multiplied in two bf16 parts.
+row's factor has more bits than its type, and fp16 does not hold what a checkpoint
+may.  Both are multiplied in two bf16 parts.
 
 Tolerance, for S = sum of |terms|: dy * row is rounded once in fp32 (2^-24); the high
 part leaves at most 2^-9 of it and the low part 2^-9 of that (2^-18); the tensor cores
@@ -80,3 +81,38 @@ def test_fp32_weights_under_autocast(dtype):
     # the kernel's own rstd is off by 4e-6 at most
     assert dw.dtype == torch.float32
     assert torch.all((dw.double() - want).abs() <= (two_parts(M) + 4e-6) * size + 2.0 ** -23 * want.abs())
+
+
+@pytest.mark.parametrize("normed", [False, True], ids=["plain", "normed"])
+@pytest.mark.parametrize("scale", [1e-9, 1e-6, 1.0, 1e6], ids=str)
+def test_fp16_gradients_with_a_checkpoint_beyond_fp16(scale, normed):
+    """Kept fp32 values that fp16 does not hold (below 2^-25, beyond 65504): the products
+    are what the formula says, in fp32 and, where the result fits, in fp16."""
+    from momentummamba_b200 import int8
+    M, N, K = 200, 40, 300
+    x, dy, row, col = make(M, N, K, torch.float32, torch.float16)
+    ck = int8.checkpoint_rows(x * scale)
+    row, col = (row, col) if normed else (None, None)
+    dw = int8.weight_grad_ckpt(dy, ck, row, col, out_dtype=torch.float32)
+    want, size = products64(dy, ck.restore(), row, col)
+    assert torch.all((dw.double() - want).abs() <= two_parts(M) * size + 2.0 ** -23 * want.abs())
+    if scale == 1.0:
+        half = int8.weight_grad_ckpt(dy, ck, row, col)
+        assert torch.equal(half, dw.half())
+
+
+def test_fp16_rows_at_the_types_own_limit():
+    """A finite fp16 tensor beside masked rows of the lowest value: dy is 0 there, and the
+    products stay finite."""
+    from momentummamba_b200 import int8
+    M, N, K = 130, 24, 160
+    x, dy, _, _ = make(M, N, K, torch.float16, torch.float16)
+    x[17] = torch.finfo(torch.float16).min
+    x[40, 130:] = 65024.0
+    dy[17] = 0
+    dy[40] *= 1e-3
+    ck = int8.checkpoint_rows(x)
+    dw = int8.weight_grad_ckpt(dy, ck, out_dtype=torch.float32)
+    want, size = products64(dy, ck.restore(), None, None)
+    assert torch.isfinite(dw).all()
+    assert torch.all((dw.double() - want).abs() <= two_parts(M) * size + 2.0 ** -23 * want.abs())
