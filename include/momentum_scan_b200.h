@@ -506,7 +506,8 @@ int mmb_norm_q8(int64_t rows, int64_t cols, int32_t x_type, const void* x, int64
  * 8-bit checkpoint of h in groups of 128 columns (q nullable: none kept):
  *   q = rint(h / s),   s = scale[row * ceil(cols / 128) + group], the smallest
  *   power of two >= 2^-100 with max|h| <= 127 s; the kept value is q * s
- *   (|q| <= 63 where s = 2^122, so that it stays finite).
+ *   (|q| <= 63 where 64 s is beyond h's type, so that it stays finite there: s =
+ *   2^122, or 2^10 where h is finite fp16).
  * rstd[row] (nullable) as above.  norm == 0 with n NULL keeps x as it is. */
 int mmb_norm_ck8_fwd(int64_t rows, int64_t cols, int32_t x_type, const void* x, int64_t ldx,
                      int32_t res_type, const void* residual, int64_t ldr, const float* weight,

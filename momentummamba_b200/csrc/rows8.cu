@@ -9,7 +9,8 @@
 //  * 8-bit checkpoints (training): h is kept in groups of 128 columns, each
 //    with the smallest power of two s (at least 2^-100) with max|h| <= 127 s:
 //        q = rint(h / s),   kept value q * s
-//    (|q| <= 63 where s = 2^122, so that it stays finite).
+//    (|q| <= 63 where 64 s is beyond h's type, so that it stays finite there: s =
+//    2^122, or 2^10 where h is finite fp16).
 //    A power of two makes h / s exact, so what is kept is the same on every
 //    run, and q * s is exact in bf16 and tf32, which the weight gradient
 //    multiplies it in.  The norm h * rstd * weight goes out beside it in the
@@ -38,6 +39,8 @@
 // 136 (90), 134 (70); these are bound by the number of accesses.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "mmb_common.cuh"
 
@@ -304,6 +307,7 @@ template <class EX, class ER, bool VEC, int NC, int NT, bool CK, int LPR = 32>
 __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
     __shared__ float2 part[R8_MAX_WARPS];
     constexpr int RPW = 32 / LPR;
+    constexpr bool F16 = std::is_same<EX, T8F16>::value, ER_F16 = std::is_same<ER, T8F16>::value;
     const int lane = threadIdx.x & (LPR - 1), warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
     const int64_t first = ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * RPW;
     if (first >= p.rows) return;  // whole warps; blocks of several warps hold one row
@@ -425,7 +429,9 @@ __global__ void __launch_bounds__(NT) r8_fwd_kernel(const R8Fwd p) {
                     float q[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) q[j] = __fmul_rn(v[c][V * g + j], inv);
-                    if (e == 122) {  // values at the type's own limit: 64 s would be 2^128
+                    bool edge = e == 122;  // values at the type's own limit: 64 s would be 2^128
+                    if constexpr (F16) edge |= e == 10 && t[g] < 65520.f && (ER_F16 || !p.res);
+                    if (edge) {
 #pragma unroll
                         for (int j = 0; j < V; ++j) q[j] = fminf(fmaxf(q[j], -63.f), 63.f);
                     }
