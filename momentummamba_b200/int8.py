@@ -392,9 +392,10 @@ def _norm_ckpt_bwd(dn, dh, weight, q, stats, out_dtype, want_dw):
         dw = torch.empty(cols, dtype=torch.float32, device=dev)
         work = torch.empty(_bwd_floats(rows, cols), dtype=torch.float32, device=dev)
         wp, kp = dw.data_ptr(), work.data_ptr()
+    weight = _weight(weight, cols)  # held until the call has been queued
     sp = stats.data_ptr()
     _call("mmb_norm_ck8_bwd", idx, rows, cols, _TYPES[dn.dtype], dn2.data_ptr(), lddn,
-          _TYPES[dx_dtype], hp, lddh, _p(_weight(weight, cols)), q.data_ptr(), q.stride(0), sp,
+          _TYPES[dx_dtype], hp, lddh, _p(weight), q.data_ptr(), q.stride(0), sp,
           sp + 4 * rows * -(-cols // GROUP), dx.data_ptr(), cols, wp, kp)
     return dx, dw
 
