@@ -400,6 +400,12 @@ def _norm_ckpt_bwd(dn, dh, weight, q, stats, out_dtype, want_dw):
     return dx, dw
 
 
+def _grad_wanted(*tensors: Optional[torch.Tensor]) -> bool:
+    """Whether autograd records this call.  Read before a Function is applied: inside its
+    forward grad mode is off, and needs_input_grad follows requires_grad alone."""
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 def _as(t: Optional[torch.Tensor], dtype) -> Optional[torch.Tensor]:
     return t if t is None or t.dtype == dtype else t.to(dtype)
 
@@ -450,7 +456,11 @@ def rms_norm_ckpt(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
 
     Arguments as in rms_norm_q8; n is in out_dtype (x's type by default), h in
     the residual's type (x itself without a residual)."""
-    out = RmsNormCkptFn.apply(x, weight, residual, eps, out_dtype or x.dtype)
+    dt = out_dtype or x.dtype
+    if not _grad_wanted(x, weight, residual):
+        n, h, _, _ = _norm_ckpt(x, weight, residual, eps, 1, dt, False, "rms_norm_ckpt")
+        return n, x if h is None else h
+    out = RmsNormCkptFn.apply(x, weight, residual, eps, dt)
     return out if residual is not None else (out, x)
 
 
@@ -534,13 +544,13 @@ def _norm_linear_ckpt_bwd(ctx, dy, dh=None):
     norm_weight, weight, q, stats = ctx.saved_tensors
     if dy is None:
         return _as(dh, xdt), None, _as(dh, rdt) if need[2] else None, None, None, None
-    rows, cols = q.shape
     dx = dnw = dw = db = None
     if need[0] or need[1] or need[2]:
         with torch.autocast("cuda", enabled=False):
             dn = torch.matmul(dy, weight.to(dy.dtype))
         dx, dnw = _norm_ckpt_bwd(dn, dh, norm_weight, q, stats, rdt or xdt, need[1])
     if need[3]:
+        rows, cols = q.shape
         sp, nw = stats.data_ptr(), _weight(norm_weight, cols)
         dw = _weight_grad(_index(dy, q, stats), dy, _TYPES[dy.dtype], q, sp,
                           sp + 4 * rows * -(-cols // GROUP), _p(nw), weight.dtype,
@@ -557,7 +567,7 @@ class NormLinearCkptFn(torch.autograd.Function):
     def forward(ctx, x, norm_weight, residual, weight, bias, eps):
         dt = _linear_types(weight.dtype)
         n, h, q, stats = _norm_ckpt(x, norm_weight, residual, eps, 1, dt,
-                                    any(ctx.needs_input_grad[:5]), "norm_linear_ckpt")
+                                    any(ctx.needs_input_grad[:4]), "norm_linear_ckpt")
         y = _linear(n, weight, bias)
         ctx.save_for_backward(norm_weight, weight, q, stats)
         ctx.meta = (x.dtype, None if residual is None else residual.dtype,
@@ -577,6 +587,10 @@ def norm_linear_ckpt(x: torch.Tensor, norm_weight: Optional[torch.Tensor], weigh
     weight's; neither h nor the norm is kept.  The product runs in the weight's
     type (autocast's where it is on); weight is (N, cols) fp32, bf16 or fp16."""
     _linear_check(x, weight, bias, "norm_linear_ckpt")
+    if not _grad_wanted(x, norm_weight, residual, weight, bias):
+        n, h, _, _ = _norm_ckpt(x, norm_weight, residual, eps, 1, _linear_types(weight.dtype), False,
+                                "norm_linear_ckpt")
+        return _linear(n, weight, bias), x if h is None else h
     out = NormLinearCkptFn.apply(x, norm_weight, residual, weight, bias, eps)
     return out if residual is not None else (out, x)
 
@@ -614,6 +628,8 @@ def linear_ckpt(x: torch.Tensor, weight: torch.Tensor,
                 bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """linear(x, weight, bias) that keeps x in 8 bits for the weight's gradient."""
     _linear_check(x, weight, bias, "linear_ckpt")
+    if not _grad_wanted(x, weight, bias):
+        return _linear(x.to(_linear_types(weight.dtype)), weight, bias)
     return LinearCkptFn.apply(x, weight, bias)
 
 

@@ -37,3 +37,40 @@ def test_a_converted_norm_weight_lives_through_the_backward_call(calls, monkeypa
     int8._norm_ckpt_bwd(torch.randn(rows, cols), None, torch.ones(cols, dtype=torch.bfloat16), q,
                         torch.zeros(rows * 2), torch.float32, True)
     assert alive == [True]
+
+
+def kept(calls):
+    """Whether each forward call was given a place for a checkpoint."""
+    return [args[16] is not None for name, args in calls if name == "mmb_norm_ck8_fwd"]
+
+
+@pytest.mark.parametrize("off", [torch.no_grad, torch.inference_mode], ids=["no_grad", "inference_mode"])
+def test_no_checkpoint_where_no_gradient_is_wanted(calls, off):
+    """Parameters that require a gradient, evaluated without one: the norm is called without
+    a checkpoint, and the plain linear makes no library call at all."""
+    x = torch.randn(4, 64)
+    w, nw = torch.randn(8, 64, requires_grad=True), torch.ones(64, requires_grad=True)
+    with off():
+        n, _ = int8.rms_norm_ckpt(x, nw)
+        y, _ = int8.norm_linear_ckpt(x, nw, w, residual=x)
+        assert kept(calls) == [False, False]
+        calls.clear()
+        z = int8.linear_ckpt(x, w)
+        assert calls == []
+    assert not n.requires_grad and not y.requires_grad and not z.requires_grad
+
+
+def test_checkpoints_where_a_gradient_is_wanted(calls):
+    x = torch.randn(4, 64)
+    w, nw = torch.randn(8, 64, requires_grad=True), torch.ones(64, requires_grad=True)
+    b = torch.zeros(8, requires_grad=True)
+    int8.rms_norm_ckpt(x, nw)
+    int8.norm_linear_ckpt(x, nw, w)
+    int8.linear_ckpt(x, w)
+    assert kept(calls) == [True] * 3
+    calls.clear()
+    # frozen tensors, a frozen weight, only the bias trained: nothing reads a checkpoint
+    int8.rms_norm_ckpt(x, nw.detach())
+    int8.norm_linear_ckpt(x, nw.detach(), w.detach(), b)[0].sum().backward()
+    int8.linear_ckpt(x.clone().requires_grad_(), w.detach())
+    assert kept(calls) == [False] * 2 and torch.equal(b.grad, torch.full((8,), 4.0))
