@@ -49,6 +49,8 @@ class Int8Block(nn.Module):
         self.in_proj, self.out_proj = Int8Linear(mixer.in_proj), Int8Linear(mixer.out_proj)
 
     def _in(self, x, residual):
+        if residual is not None and residual.dtype not in (x.dtype, torch.float32):
+            residual = residual.float()  # a 16-bit input to an fp32 model: the stream widens
         n, h = rms_norm_q8(x, None if self.norm.use_mup else self.norm.weight, residual=residual,
                            eps=self.norm.eps)
         return self.in_proj(n, self.mixer.x_proj.weight.dtype), h
