@@ -26,7 +26,10 @@ from .mamba_momentum import MambaMomentum, MambaMomentumBlock
 
 
 class Int8Linear(nn.Module):
-    """A linear's weight as 8-bit rows (one scale an output channel) and its bias."""
+    """A linear's weight as 8-bit rows (one scale an output channel) and its bias.
+
+    Scales and bias are fp32 whatever type the module is moved to: .to(torch.bfloat16)
+    or .half() changes what the model computes around the products, not the weights."""
 
     def __init__(self, linear: nn.Linear):
         super().__init__()
@@ -35,6 +38,15 @@ class Int8Linear(nn.Module):
         self.register_buffer("scale", w.scale)
         self.register_buffer("bias", None if linear.bias is None
                              else linear.bias.detach().float().clone())
+
+    def _apply(self, fn, recurse=True):
+        held = {"scale": self.scale, "bias": self.bias}
+        super()._apply(fn, recurse)
+        for name, old in held.items():
+            new = getattr(self, name)
+            if new is not None and new.dtype != torch.float32:
+                setattr(self, name, old.to(new.device))
+        return self
 
     def forward(self, x: Q8Rows, out_dtype: torch.dtype) -> torch.Tensor:
         return linear_q8(x, Q8Rows(self.q, self.scale), self.bias, out_dtype=out_dtype)

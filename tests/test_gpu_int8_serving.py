@@ -43,3 +43,20 @@ def test_16_bit_inputs_to_an_fp32_model(dtype):
     ya, _ = m8.step(x[:, 0], caches(m, 2))
     yb, _ = m8.step(x[:, 0].float(), caches(m, 2))
     assert ya.dtype == torch.float32 and torch.equal(ya, yb)
+
+
+def test_moving_to_another_type_leaves_the_8_bit_weights_alone():
+    m = model(d_model=128, bias=True)
+    x = torch.randn(2, 40, 128, device=DEV)
+    with torch.no_grad():
+        want = m(x)
+    m8 = served(m)
+    before = {k: v.clone() for k, v in m8.state_dict().items() if "proj" in k and "mixer" not in k}
+    m8 = m8.to(torch.bfloat16)
+    y = m8(x.bfloat16())
+    assert y.dtype == torch.bfloat16
+    assert rel(y.float() - x, want - x) <= 6e-2 + 3e-2    # 8 bits, and bf16 activations on top
+    for back in (m8.half(), m8.float(), m8.cpu().to(DEV, torch.bfloat16)):
+        after = back.state_dict()
+        for k, v in before.items():
+            assert after[k].dtype == v.dtype and torch.equal(after[k], v), k
