@@ -9,13 +9,16 @@ Between the blocks only the residual stream is stored in full: each block adds
 its predecessor's output to it, norms the sum and emits 8-bit rows in one kernel
 (rms_norm_q8).  The conv, the scan and the two small projections (x_proj,
 dt_proj: the recurrence's step sizes and B, C, which 8 bits would disturb most)
-run as in the model, on its parameters.  The weights held in 8 bits take a
-quarter of their fp32 size; a decoding step reads little else.
+run as in the model.  What is served is a copy of the model as it is now: the
+two projections in 8 bits alone, a quarter of their fp32 size, the rest in full.
+Later changes to the model do not reach it, nor does .to() on it reach the model.
 
 No reference counterpart (the reference serves in fp32).  Inference only: no
 gradients.
 """
 from __future__ import annotations
+
+import copy
 
 import torch
 import torch.nn as nn
@@ -34,7 +37,10 @@ class Int8Linear(nn.Module):
     def __init__(self, linear: nn.Linear):
         super().__init__()
         w = quantize_rows(linear.weight.detach())
-        self.register_buffer("q", w.q)
+        # contiguous rows of a multiple of 16 bytes: copies and moves keep the alignment that
+        # the product's loads need
+        self.in_features = w.q.shape[1]
+        self.register_buffer("q", nn.functional.pad(w.q, (0, -self.in_features % 16)))
         self.register_buffer("scale", w.scale)
         self.register_buffer("bias", None if linear.bias is None
                              else linear.bias.detach().float().clone())
@@ -49,15 +55,17 @@ class Int8Linear(nn.Module):
         return self
 
     def forward(self, x: Q8Rows, out_dtype: torch.dtype) -> torch.Tensor:
-        return linear_q8(x, Q8Rows(self.q, self.scale), self.bias, out_dtype=out_dtype)
+        q = self.q if self.q.shape[1] == self.in_features else self.q[:, :self.in_features]
+        return linear_q8(x, Q8Rows(q, self.scale), self.bias, out_dtype=out_dtype)
 
 
 class Int8Block(nn.Module):
-    """One residual block; holds the model's own mixer for what stays in full."""
+    """One residual block; mixer holds what stays in full: all but the two projections."""
 
     def __init__(self, norm, mixer: MambaMomentumBlock):
         super().__init__()
-        self.norm, self.mixer = norm, mixer
+        self.norm = copy.deepcopy(norm)
+        self.mixer = copy.deepcopy(mixer, {id(mixer.in_proj): None, id(mixer.out_proj): None})
         self.in_proj, self.out_proj = Int8Linear(mixer.in_proj), Int8Linear(mixer.out_proj)
 
     def _in(self, x, residual):

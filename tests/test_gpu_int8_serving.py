@@ -60,3 +60,44 @@ def test_moving_to_another_type_leaves_the_8_bit_weights_alone():
         after = back.state_dict()
         for k, v in before.items():
             assert after[k].dtype == v.dtype and torch.equal(after[k], v), k
+
+
+def test_no_full_projection_weights_are_held():
+    m = model(d_model=96, bias=True)
+    m8 = served(m)
+    c = m.config
+    full = {2 * c.d_inner * c.d_model, c.d_inner * c.d_model}
+    for name, t in m8.state_dict().items():
+        assert t.dtype == torch.int8 or t.numel() not in full, name
+    assert not any(p.numel() in full for p in m8.parameters())
+    # neither does a conversion of what is served reach the model, nor training it what is served
+    x = torch.randn(2, 9, 96, device=DEV)
+    y = m8(x)
+    with torch.no_grad():
+        for p in m.parameters():
+            p.add_(1)
+    assert torch.equal(m8(x), y)
+    m8.bfloat16()
+    assert all(p.dtype == torch.float32 for p in m.parameters())
+
+
+@pytest.mark.parametrize("d_model", [75, 96])
+def test_copies_keep_the_rows_alignment(d_model, monkeypatch):
+    """d_model 75: rows of 75 and 150 values.  No product copies its weight first, before
+    or after the module has been copied, saved and loaded."""
+    import copy
+
+    from momentummamba_b200 import int8
+    m = model(d_model=d_model, n_layers=1)
+    x = torch.randn(2, 9, d_model, device=DEV)
+    first = served(m)
+    y = first(x)
+    clone = copy.deepcopy(first).cpu().to(DEV)
+    loaded = served(model(d_model=d_model, n_layers=1, seed=5))
+    loaded.load_state_dict({k: v.clone() for k, v in first.state_dict().items()})
+    taken = []
+    rows = int8._tma_rows
+    monkeypatch.setattr(int8, "_tma_rows", lambda t: taken.append((t, rows(t))) or taken[-1][1])
+    for m8 in (first, clone, loaded):
+        assert torch.equal(m8(x), y)
+    assert len(taken) == 3 * 4 and all(out[2] is t for t, out in taken)
