@@ -135,7 +135,7 @@ class ResidualBlock(nn.Module):
         self.norm = RMSNorm(config.d_model, config.rms_norm_eps, config.mup)
 
     def forward(self, x):
-        if self.mixer.config.act_ckpt == "int8":
+        if getattr(getattr(self.mixer, "config", None), "act_ckpt", "none") == "int8":
             out, h = self.forward_ckpt(x, None)
             return out + h
         return self.mixer(self.norm(x)) + x

@@ -74,3 +74,13 @@ def test_checkpoints_where_a_gradient_is_wanted(calls):
     int8.norm_linear_ckpt(x, nw.detach(), w.detach(), b)[0].sum().backward()
     int8.linear_ckpt(x.clone().requires_grad_(), w.detach())
     assert kept(calls) == [False] * 2 and torch.equal(b.grad, torch.full((8,), 4.0))
+
+
+def test_a_block_takes_a_mixer_without_a_config():
+    """A mixer replaced by any module: the block calls it, as it did before there were
+    checkpoints."""
+    from momentummamba_b200.mamba_momentum import MambaMomentumConfig, ResidualBlock
+    block = ResidualBlock(MambaMomentumConfig(d_model=16, n_layers=1))
+    block.mixer = torch.nn.Identity()
+    x = torch.randn(2, 3, 16)
+    assert torch.equal(block(x), block.norm(x) + x)
