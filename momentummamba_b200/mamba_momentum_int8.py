@@ -12,6 +12,8 @@ dt_proj: the recurrence's step sizes and B, C, which 8 bits would disturb most)
 run as in the model.  What is served is a copy of the model as it is now: the
 two projections in 8 bits alone, a quarter of their fp32 size, the rest in full.
 Later changes to the model do not reach it, nor does .to() on it reach the model.
+Blocks, norms, mixers and projections that have been replaced or hooked are
+refused: their weights alone do not say what they compute.
 
 No reference counterpart (the reference serves in fp32).  Inference only: no
 gradients.
@@ -25,7 +27,14 @@ import torch.nn as nn
 
 from .conv import conv1d_step
 from .int8 import Q8Rows, linear_q8, quantize_rows, rms_norm_q8
-from .mamba_momentum import MambaMomentum, MambaMomentumBlock
+from .mamba_momentum import MambaMomentum, MambaMomentumBlock, ResidualBlock, RMSNorm, runs_as
+
+
+def _ordinary(module, cls, name):
+    if not runs_as(module, cls):
+        raise ValueError(f"Int8MambaMomentum: {name} must be an ordinary {cls.__name__} without hooks, "
+                         f"got {type(module).__name__} (merge adapters and remove hooks first)")
+    return module
 
 
 class Int8Linear(nn.Module):
@@ -62,8 +71,13 @@ class Int8Linear(nn.Module):
 class Int8Block(nn.Module):
     """One residual block; mixer holds what stays in full: all but the two projections."""
 
-    def __init__(self, norm, mixer: MambaMomentumBlock):
+    def __init__(self, block: ResidualBlock):
         super().__init__()
+        _ordinary(block, ResidualBlock, "a block")
+        norm = _ordinary(block.norm, RMSNorm, "norm")
+        mixer = _ordinary(block.mixer, MambaMomentumBlock, "mixer")
+        _ordinary(mixer.in_proj, nn.Linear, "in_proj")
+        _ordinary(mixer.out_proj, nn.Linear, "out_proj")
         self.norm = copy.deepcopy(norm)
         self.mixer = copy.deepcopy(mixer, {id(mixer.in_proj): None, id(mixer.out_proj): None})
         self.in_proj, self.out_proj = Int8Linear(mixer.in_proj), Int8Linear(mixer.out_proj)
@@ -96,7 +110,7 @@ class Int8MambaMomentum(nn.Module):
     def __init__(self, model: MambaMomentum):
         super().__init__()
         self.config = model.config
-        self.layers = nn.ModuleList([Int8Block(b.norm, b.mixer) for b in model.layers])
+        self.layers = nn.ModuleList([Int8Block(b) for b in model.layers])
 
     @torch.no_grad()
     def forward(self, x):

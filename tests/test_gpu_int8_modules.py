@@ -99,3 +99,18 @@ def test_a_parametrized_weight():
     for k in (m, m8):
         nn.utils.parametrize.register_parametrization(k.layers[1].mixer.out_proj, "weight", Twice())
     compare(m, m8)
+
+
+@pytest.mark.parametrize("name", PARTS)
+def test_serving_refuses_what_its_weights_do_not_say(name):
+    from momentummamba_b200.mamba_momentum_int8 import Int8MambaMomentum
+    m = model()
+    handle = part(m, name).register_forward_hook(lambda mod, args, out: None)
+    with pytest.raises(ValueError, match="without hooks"):
+        Int8MambaMomentum(m)
+    handle.remove()
+    Int8MambaMomentum(m)
+    if name.endswith("proj"):
+        setattr(m.layers[1].mixer, name, Adapted(part(m, name)))
+        with pytest.raises(ValueError, match=f"{name} must be an ordinary Linear"):
+            Int8MambaMomentum(m)
