@@ -43,8 +43,9 @@ _TYPES = {torch.float32: _lib.MMB_F32, torch.bfloat16: _lib.MMB_BF16, torch.floa
 # A decoding step's kernels take a few microseconds, so its calls are held to a few
 # too: the raw stream handle (torch.cuda.current_stream() builds an object, 3 us), one
 # tensor for the small outputs of a call, sizes given one by one.
-_raw_stream = torch._C._cuda_getCurrentRawStream
-_get_device = torch._C._cuda_getDevice
+# A torch without CUDA has neither, and no call gets that far there.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_get_device = getattr(torch._C, "_cuda_getDevice", None)
 
 
 def _type(t: torch.Tensor, what: str) -> int:

@@ -84,3 +84,20 @@ def test_a_block_takes_a_mixer_without_a_config():
     block.mixer = torch.nn.Identity()
     x = torch.randn(2, 3, 16)
     assert torch.equal(block(x), block.norm(x) + x)
+
+
+def test_the_model_imports_where_torch_has_no_cuda():
+    """A torch built without CUDA lacks the stream and device entry points: models are
+    still built, saved and loaded there."""
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for name in [n for n in vars(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "from momentummamba_b200.mamba_momentum import MambaMomentum, MambaMomentumConfig\n"
+            "import momentummamba_b200.mamba_momentum_int8, momentummamba_b200.LinOSS_pytorch\n"
+            "MambaMomentum(MambaMomentumConfig(d_model=16, n_layers=1)).state_dict()\n")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    run = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True)
+    assert run.returncode == 0, run.stderr[-2000:]
