@@ -136,6 +136,36 @@ __device__ __forceinline__ uint32_t w8_pack2(float a, float b) {
     const __nv_bfloat162 t = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&t);
 }
+// Two values as PARTS bf16 pairs whose sum they are.  From W8_EDGE on the nearest
+// bf16 would be an infinity and the next part its opposite: the largest finite value
+// is taken there, and an infinity or a NaN stands alone.
+constexpr float W8_EDGE = 0x1.ffp127f, W8_BF16_MAX = 0x1.fep127f;
+template <int PARTS>
+__device__ __forceinline__ void w8_parts(float2 v, uint32_t (&o)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        o[i] = w8_pack2(v.x, v.y);
+        v.x -= bf16_lo(o[i]);
+        v.y -= bf16_hi(o[i]);
+    }
+}
+template <int PARTS>
+__device__ __forceinline__ void w8_parts_edge(float2 v, uint32_t (&o)[PARTS]) {
+    const auto high = [](float x) {
+        return fabsf(x) < INFINITY ? fminf(fmaxf(x, -W8_BF16_MAX), W8_BF16_MAX) : x;
+    };
+    const auto rest = [](float x, float h) { return fabsf(x) < INFINITY ? x - h : 0.f; };
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        o[i] = w8_pack2(high(v.x), high(v.y));
+        v.x = rest(v.x, bf16_lo(o[i]));
+        v.y = rest(v.y, bf16_hi(o[i]));
+    }
+}
+__device__ __forceinline__ float w8_top(float top, float2 v) {
+    return fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+}
+
 // `bar` counts an arrival of this lane once its cp.async copies so far have landed
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar))
@@ -435,79 +465,106 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 // steps: 2^15 times them would be an infinity
                 if (__any_sync(0xffffffffu, huge)) widen(0x1p-32f, 0x1p32f);
                 else widen(1.f, 1.f);
+                // dy * row in bf16 parts.  A block with values at fp32's own limit is split a
+                // second time, with care
                 if constexpr (D::F32) {
-                    // dy * row = high + middle + low, each bf16: 4 columns of either
-                    // block of 64 a step (16 lanes then cover a row of each)
+                    // high, middle and low: 4 columns of either block of 64 a step (16 lanes
+                    // then cover a row of each)
                     const int c = ct & 15;
-                    constexpr int STEPS = BT * BN / 8 / CT;
+                    constexpr int STEPS = BT * BN / 8 / CT, AT_ONCE = 4;
+                    static_assert(STEPS % AT_ONCE == 0, "whole batches");
                     const uint32_t ds = smem_u32(slot_dy(s)) + c * 16;
-                    uint4 x[STEPS][2];
-                    float r[STEPS];
+                    const auto split = [&](const uint4& x, float r, int t, int h, auto parts) {
+                        const uint32_t dst = as + Sm::A + w8_chunk<BT>(h, t, c >> 1) + (c & 1) * 8;
+                        const float2 v0 = fmul2(
+                            make_float2(__uint_as_float(x.x), __uint_as_float(x.y)), f2(r));
+                        const float2 v1 = fmul2(
+                            make_float2(__uint_as_float(x.z), __uint_as_float(x.w)), f2(r));
+                        uint32_t o0[3], o1[3];
+                        parts(v0, o0);
+                        parts(v1, o1);
 #pragma unroll
-                    for (int i = 0; i < STEPS; ++i) {
-                        const int t = (ct >> 4) + i * (CT / 16);
-                        x[i][0] = lds16(ds + t * (BN * 4));
-                        x[i][1] = lds16(ds + t * (BN * 4) + 256);
-                        r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
+                        for (int i = 0; i < 3; ++i) sts8(dst + i * Sm::P1, o0[i], o1[i]);
+                    };
+                    float top = 0.f;
+#pragma unroll
+                    for (int i0 = 0; i0 < STEPS; i0 += AT_ONCE) {
+                        uint4 x[AT_ONCE][2];
+                        float r[AT_ONCE];
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i) {
+                            const int t = (ct >> 4) + (i0 + i) * (CT / 16);
+                            x[i][0] = lds16(ds + t * (BN * 4));
+                            x[i][1] = lds16(ds + t * (BN * 4) + 256);
+                            r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
+                        }
+#pragma unroll
+                        for (int i = 0; i < AT_ONCE; ++i)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h)
+                                split(x[i][h], r[i], (ct >> 4) + (i0 + i) * (CT / 16), h,
+                                      [&](float2 v, uint32_t (&o)[3]) {
+                                          top = w8_top(top, v);
+                                          w8_parts<3>(v, o);
+                                      });
                     }
-#pragma unroll
-                    for (int i = 0; i < STEPS; ++i) {
-                        const int t = (ct >> 4) + i * (CT / 16);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const uint32_t dst =
-                                as + Sm::A + w8_chunk<BT>(h, t, c >> 1) + (c & 1) * 8;
-                            float2 v0 = make_float2(__uint_as_float(x[i][h].x),
-                                                    __uint_as_float(x[i][h].y));
-                            float2 v1 = make_float2(__uint_as_float(x[i][h].z),
-                                                    __uint_as_float(x[i][h].w));
-                            v0 = fmul2(v0, f2(r[i]));
-                            v1 = fmul2(v1, f2(r[i]));
-#pragma unroll
-                            for (int part = 0; part < 3; ++part) {
-                                const uint32_t o0 = w8_pack2(v0.x, v0.y), o1 = w8_pack2(v1.x, v1.y);
-                                sts8(dst + part * Sm::P1, o0, o1);
-                                v0.x -= bf16_lo(o0);
-                                v0.y -= bf16_hi(o0);
-                                v1.x -= bf16_lo(o1);
-                                v1.y -= bf16_hi(o1);
-                            }
+                    if (__any_sync(0xffffffffu, top >= W8_EDGE)) {
+#pragma unroll 1
+                        for (int i = 0; i < 2 * STEPS; ++i) {
+                            const int t = (ct >> 4) + (i >> 1) * (CT / 16), h = i & 1;
+                            split(lds16(ds + t * (BN * 4) + h * 256),
+                                  p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f, t, h,
+                                  [](float2 v, uint32_t (&o)[3]) { w8_parts_edge<3>(v, o); });
                         }
                     }
                 }
                 if constexpr (D::PARTS == 2) {
-                    // dy * row = high + low, each bf16: 8 neighbouring lanes take the 128
-                    // bytes of a block of 64 columns of one token
+                    // high and low: 8 neighbouring lanes take the 128 bytes of a block of 64
+                    // columns of one token
                     const int c = ct & 7;
                     constexpr int ITEMS = BT * (BN / 64), STEPS = ITEMS / (CT / 8), AT_ONCE = 4;
                     static_assert(STEPS % AT_ONCE == 0, "whole batches");
                     const uint32_t ds = smem_u32(slot_dy(s)) + c * 16;
+                    const auto load = [&](int i, uint4& x, float& r) {
+                        const int item = (ct >> 3) + i * (CT / 8);
+                        const int t = item / (BN / 64), h = item % (BN / 64);
+                        x = lds16(ds + t * (BN * 2) + h * 128);
+                        r = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
+                    };
+                    const auto split = [&](int i, const uint4& x, float r, auto parts) {
+                        const int item = (ct >> 3) + i * (CT / 8);
+                        const int t = item / (BN / 64), h = item % (BN / 64);
+                        const uint32_t xs[4] = {x.x, x.y, x.z, x.w};
+                        uint32_t o[4][2];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) parts(fmul2(D::dy2(xs[e]), f2(r)), o[e]);
+                        const uint32_t dst = as + Sm::A + w8_chunk<BT>(h, t, c);
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+                            sts16(dst + k * Sm::P1, make_uint4(o[0][k], o[1][k], o[2][k], o[3][k]));
+                    };
+                    float top = 0.f;
 #pragma unroll
                     for (int i0 = 0; i0 < STEPS; i0 += AT_ONCE) {
                         uint4 x[AT_ONCE];
                         float r[AT_ONCE];
 #pragma unroll
-                        for (int i = 0; i < AT_ONCE; ++i) {
-                            const int item = (ct >> 3) + (i0 + i) * (CT / 8);
-                            const int t = item / (BN / 64), h = item % (BN / 64);
-                            x[i] = lds16(ds + t * (BN * 2) + h * 128);
-                            r[i] = p.row ? lds4f(fs + 4 * (ROW + t)) : 1.f;
-                        }
+                        for (int i = 0; i < AT_ONCE; ++i) load(i0 + i, x[i], r[i]);
 #pragma unroll
-                        for (int i = 0; i < AT_ONCE; ++i) {
-                            const int item = (ct >> 3) + (i0 + i) * (CT / 8);
-                            const int t = item / (BN / 64), h = item % (BN / 64);
-                            const uint32_t xs[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                            uint32_t hi[4], lo[4];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float2 v = fmul2(D::dy2(xs[e]), f2(r[i]));
-                                hi[e] = w8_pack2(v.x, v.y);
-                                lo[e] = w8_pack2(v.x - bf16_lo(hi[e]), v.y - bf16_hi(hi[e]));
-                            }
-                            const uint32_t dst = as + Sm::A + w8_chunk<BT>(h, t, c);
-                            sts16(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-                            sts16(dst + Sm::P1, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                        for (int i = 0; i < AT_ONCE; ++i)
+                            split(i0 + i, x[i], r[i], [&](float2 v, uint32_t (&o)[2]) {
+                                top = w8_top(top, v);
+                                w8_parts<2>(v, o);
+                            });
+                    }
+                    if (__any_sync(0xffffffffu, top >= W8_EDGE)) {
+#pragma unroll 1
+                        for (int i = 0; i < STEPS; ++i) {
+                            uint4 x;
+                            float r;
+                            load(i, x, r);
+                            split(i, x, r,
+                                  [](float2 v, uint32_t (&o)[2]) { w8_parts_edge<2>(v, o); });
                         }
                     }
                 }
