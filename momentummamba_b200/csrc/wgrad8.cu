@@ -14,7 +14,7 @@
 //   * bf16 dy without `row` goes from TMA to the tensor cores as it is.
 //   * otherwise dy (times row, in fp32) is split into bf16 parts: 16-bit dy into
 //     two (16 bits: exact without row, with it off by at most 2^-17 of a term; one
-//     part would be off by 2^-9, as much as a bf16 result's own rounding), fp32 dy
+//     part would be off by up to 2^-8, as much as a bf16 result's own rounding), fp32 dy
 //     into three (24 bits), the high part into one accumulator and the two small
 //     ones into another.  fp16 dy is not multiplied as it is, since fp16 does not
 //     hold what a checkpoint may: kept values reach from 2^-100 to fp32's largest.
@@ -69,8 +69,7 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 // AG: checkpoint groups (128 columns) of a tile; BN: its dy columns; BT: tokens of
 // a block; RL, RC: blocks in flight as they lie in memory / widened; RA:
 // accumulators; CW, EW: converter (in CG groups, each at a block of its own) and
-// epilogue warps; SEG: token blocks that accumulate in TMEM before the sums move
-// to registers.
+// epilogue warps.
 //
 // Two groups share each load of dy (65536 x (4096, 1024) bf16: 815 -> 560 us).
 //
@@ -85,18 +84,26 @@ template <int GROUPS>
 struct W8Half {
     static constexpr bool F32 = false;
     static constexpr int PARTS = 1;  // dy as it is
-    static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2, SEG = 1 << 30;
+    static constexpr int AG = GROUPS, BN = 256, BT = 64, BYTES = 2;
     static constexpr int RL = AG == 1 ? 4 : 3, RC = AG == 1 ? 3 : 2, RA = AG == 1 ? 2 : 1;
     static constexpr int CW = 8, CG = 1, EW = 8;
 };
 // The tensor cores' fp32 accumulation truncates: its error grows with the number
-// of steps.  1024 tokens (64 steps) at a time, added to sums in registers with
-// ordinary rounding, and the small parts in an accumulator of their own, keep
-// the result as near as an fp32 product's.
+// of steps, so every so many tokens the sums leave TMEM and are added up with
+// ordinary rounding.
+//   * fp32 dy: 1024 tokens, added in registers, with the small parts in an
+//     accumulator of their own: 2e-7 against 64 bits, nearer than an fp32 product.
+//   * 16-bit dy, whose tiles are too large for registers: added where the result
+//     goes, in fp32.  Against 64 bits, random values: an fp32 result of bf16 dy is off
+//     by 1e-6 with 4096 tokens, 2.5e-6 with 8192 and 1.6e-5 with 32768, with dy in two
+//     parts by 6e-6, 1.1e-5 and 3.5e-5; 65536 x (4096, 1024) takes 565 us, 505 and 475
+//     (905, 870 and 860).  A 16-bit result is off by its own 1.65e-3 or 2.05e-4 in any
+//     case, and gathers 32768 tokens.
+constexpr int W8_SEG_FP32_DY = 1024, W8_SEG_FP32_DW = 4096, W8_SEG_16_DW = 32768;
 struct W8F32 {
     static constexpr bool F32 = true;
     static constexpr int PARTS = 3;
-    static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4, SEG = 32;
+    static constexpr int AG = 1, BN = 128, BT = 32, BYTES = 4;
     static constexpr int RL = 4, RC = 4, RA = 2, CW = 8, CG = 4, EW = 8;
 };
 // 16-bit dy (bf16 or fp16 in memory: BF) in two bf16 parts.  Blocks of 32 tokens
@@ -107,7 +114,7 @@ template <bool BF, int GROUPS>
 struct W8Two {
     static constexpr bool F32 = false;
     static constexpr int PARTS = 2;
-    static constexpr int AG = GROUPS, BN = 256, BT = 32, BYTES = 2, SEG = 1 << 30;
+    static constexpr int AG = GROUPS, BN = 256, BT = 32, BYTES = 2;
     static constexpr int RL = 3, RC = AG == 1 ? 4 : 3, RA = AG == 1 ? 2 : 1;
     static constexpr int CW = 8, CG = 2, EW = 8;
     // two values of dy in fp32
@@ -180,11 +187,13 @@ struct W8Params {
     int64_t groups;
     const float* row;  // nullable
     const float* col;  // nullable
-    void* dw;          // one slice: the result itself
+    void* dw;
     int64_t ldw;
     int out_type;
-    float* work;  // more slices: (slices, N, ldp) partial sums
+    float* work;  // (slices, N, ldp) partial sums
     int64_t ldp;
+    int in_work;  // the result goes through work
+    int seg;      // token blocks that accumulate in TMEM before the sums leave it
     int dy_blocks, q_blocks;  // tensor maps by column blocks: one box a tile (see w8_launch)
     int* err;
 };
@@ -355,9 +364,9 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 int64_t k0, n0, b0;
                 int nb;
                 unit_of(u, k0, n0, b0, nb);
+                int in_seg = 0;
                 for (int b = 0; b < nb; ++b, rl.next(), rc.next()) {
                     const int a = ra.s;
-                    const int in_seg = b % D::SEG;
                     if (in_seg == 0) {
                         ok = ws_wait(&acc_empty[a], ra.ph ^ 1u, abort, p.err);
                         if (!ok) break;
@@ -395,9 +404,10 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     }
                     if constexpr (D::PARTS == 1) umma_commit(&free_l[s]);
                     umma_commit(&free_c[c]);
-                    if (in_seg == D::SEG - 1 || b == nb - 1) {
+                    if (++in_seg == p.seg || b == nb - 1) {
                         umma_commit(&acc_full[a]);
                         ra.next();
+                        in_seg = 0;
                     }
                 }
             }
@@ -586,19 +596,33 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
             int nb;
             unit_of(u, k0, n0, b0, nb);
             const int ncols = (int)min64(p.N - n0, BN);
-            float* slice = p.slices > 1 ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k0 : nullptr;
-            // V columns n0 + c .. of this lane's column k
-            const auto put = [&](int g, int c, const auto& v) {
+            float* slice = p.in_work ? p.work + ((u / tiles) * p.N + n0) * p.ldp + k0 : nullptr;
+            // V columns n0 + c .. of this lane's column k; every segment but the first adds
+            // to the sums that this thread left there (in fp32: w8_launch)
+            const auto put = [&](int g, int c, auto& v, bool first, bool last) {
                 constexpr int V = sizeof(v) / sizeof(v[0]);
                 const int kr = g * W8_BK + q * 32 + lane;
                 if (k0 + kr >= p.K) return;
+                if (!first) {
+                    const int64_t ld = slice ? p.ldp : p.ldw;
+                    const float* o = slice ? slice + c * p.ldp + kr
+                                           : static_cast<const float*>(p.dw) + (n0 + c) * p.ldw + k0 + kr;
+#pragma unroll
+                    for (int i0 = 0; i0 < V; i0 += 16) {
+                        float old[16];
+#pragma unroll
+                        for (int i = 0; i < 16; ++i, o += ld) old[i] = c + i0 + i < ncols ? *o : 0.f;
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) v[i0 + i] += old[i];
+                    }
+                }
                 if (slice) {
                     float* w = slice + c * p.ldp + kr;
 #pragma unroll
                     for (int i = 0; i < V; ++i, w += p.ldp)
                         if (c + i < ncols) *w = v[i];
                 } else {
-                    const float cs = p.col ? p.col[k0 + kr] : 1.f;
+                    const float cs = p.col && last ? p.col[k0 + kr] : 1.f;
                     int64_t at = (n0 + c) * p.ldw + k0 + kr;
 #pragma unroll
                     for (int i = 0; i < V; ++i, at += p.ldw)
@@ -609,7 +633,7 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                 float sum[COLS];
 #pragma unroll
                 for (int i = 0; i < COLS; ++i) sum[i] = 0.f;
-                for (int b = 0; b < nb; b += D::SEG, ra.next()) {
+                for (int b = 0; b < nb; b += p.seg, ra.next()) {
                     const int a = ra.s;
                     ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
                     if (!ok) break;
@@ -629,24 +653,26 @@ __global__ void __launch_bounds__(w8_threads<D>(), 1)
                     warp_arrive(&acc_empty[a]);
                 }
                 if (!ok) break;
-                put(0, col0, sum);
+                put(0, col0, sum, true, true);
             } else {
-                const int a = ra.s;
-                ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
-                if (!ok) break;
-                ra.next();
-                tc_fence_after();
-                const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC);
+                for (int b = 0; b < nb; b += p.seg, ra.next()) {
+                    const int a = ra.s;
+                    ok = __all_sync(0xffffffffu, ws_wait(&acc_full[a], ra.ph, abort, p.err));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint32_t trow = tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(a * ACC);
 #pragma unroll 1
-                for (int gc = 0; gc < AG * COLS; gc += 32) {
-                    const int g = gc / COLS, c = col0 + gc % COLS;
-                    float v[32];
-                    tmem_ld32(trow + (uint32_t)(g * BN + c), v);
-                    put(g, c, v);
-                    __syncwarp();
+                    for (int gc = 0; gc < AG * COLS; gc += 32) {
+                        const int g = gc / COLS, c = col0 + gc % COLS;
+                        float v[32];
+                        tmem_ld32(trow + (uint32_t)(g * BN + c), v);
+                        put(g, c, v, b == 0, nb - b <= p.seg);
+                        __syncwarp();
+                    }
+                    tc_fence_before();
+                    warp_arrive(&acc_empty[a]);
                 }
-                tc_fence_before();
-                warp_arrive(&acc_empty[a]);
+                if (!ok) break;
             }
         }
     }
@@ -733,10 +759,27 @@ template <class One, class Two>
 static bool w8_two_groups(int64_t M, int64_t N, int64_t K) {
     return w8_plan<Two>(M, N, K).us < w8_plan<One>(M, N, K).us;
 }
+// Tokens that accumulate in TMEM: its fp32 accumulation truncates, so its error grows
+// with their number.
+template <class D>
+static int w8_seg(int out_type) {
+    return (D::F32 ? W8_SEG_FP32_DY : out_type == MMB_F32 ? W8_SEG_FP32_DW : W8_SEG_16_DW) / D::BT;
+}
+// Several slices, or sums that leave TMEM more than once and have no fp32 result to
+// gather in, go through the workspace.
+template <class D>
+static bool w8_in_work(const W8Plan& plan, int out_type) {
+    return plan.slices > 1 || (!D::F32 && out_type != MMB_F32 && plan.blocks > w8_seg<D>(out_type));
+}
+template <class D>
+static int64_t w8_work_slices(int64_t M, int64_t N, int64_t K) {
+    const W8Plan plan = w8_plan<D>(M, N, K);
+    return w8_in_work<D>(plan, MMB_BF16) ? plan.slices : 0;
+}
 template <class One, class Two>
-static int64_t w8_slices(int64_t M, int64_t N, int64_t K) {
-    return w8_two_groups<One, Two>(M, N, K) ? w8_plan<Two>(M, N, K).slices
-                                            : w8_plan<One>(M, N, K).slices;
+static int64_t w8_work_slices(int64_t M, int64_t N, int64_t K) {
+    return w8_two_groups<One, Two>(M, N, K) ? w8_work_slices<Two>(M, N, K)
+                                            : w8_work_slices<One>(M, N, K);
 }
 static int64_t w8_pitch(int64_t K) { return (K + 3) / 4 * 4; }
 
@@ -747,7 +790,9 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     p.slices = plan.slices;
     p.blocks = plan.blocks;
     p.ldp = w8_pitch(p.K);
-    if (p.slices > 1 && !p.work) return MMB_ERR_WORKSPACE;
+    p.seg = w8_seg<D>(p.out_type);
+    p.in_work = w8_in_work<D>(plan, p.out_type);
+    if (p.in_work && !p.work) return MMB_ERR_WORKSPACE;
     W8Maps maps;
     // dy that is multiplied as it is and a pair of groups as (column in a block, token,
     // block) where their widths are whole blocks: one copy a tile instead of one a block
@@ -772,7 +817,7 @@ static int w8_launch(W8Params p, const void* dy, int64_t lddy, const int8_t* q, 
     const int64_t units = (p.K + kt - 1) / kt * ((p.N + D::BN - 1) / D::BN) * p.slices;
     w8_kernel<D><<<(unsigned)min64(units, 148), w8_threads<D>(), W8Smem<D>::BYTES, s>>>(p, maps);
     const int rc = mmb_launch_status();
-    if (rc != MMB_OK || p.slices == 1) return rc;
+    if (rc != MMB_OK || !p.in_work) return rc;
     const int64_t quads = p.N * (p.ldp / 4);
     const unsigned groups = p.slices >= 2 * W8_SUM_GROUPS ? W8_SUM_GROUPS : 1;
     const unsigned nq = W8_SUM_NT / groups;
@@ -796,17 +841,17 @@ extern "C" size_t mmb_wgrad_ck8_work_floats(int64_t M, int64_t N, int64_t K, int
     if (M <= 0 || N <= 0 || K <= 0 || M > INT32_MAX || N > INT32_MAX || K > INT32_MAX) return 0;
     int64_t slices;
     if (dy_type == MMB_F32) {
-        slices = w8_plan<W8F32>(M, N, K).slices;
+        slices = w8_work_slices<W8F32>(M, N, K);
     } else {
         // bf16 and fp16 in two parts share a plan; bf16 without a row factor has its own,
         // and whether there is one is not known here
-        slices = w8_slices<W8Two<true, 1>, W8Two<true, 2>>(M, N, K);
+        slices = w8_work_slices<W8Two<true, 1>, W8Two<true, 2>>(M, N, K);
         if (dy_type == MMB_BF16) {
-            const int64_t one = w8_slices<W8Half<1>, W8Half<2>>(M, N, K);
+            const int64_t one = w8_work_slices<W8Half<1>, W8Half<2>>(M, N, K);
             slices = slices > one ? slices : one;
         }
     }
-    return slices > 1 ? (size_t)slices * (size_t)N * (size_t)w8_pitch(K) : 0;
+    return (size_t)slices * (size_t)N * (size_t)w8_pitch(K);
 }
 
 extern "C" int mmb_wgrad_ck8(int64_t M, int64_t N, int64_t K, int32_t dy_type, const void* dy,
