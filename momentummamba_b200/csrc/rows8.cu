@@ -498,9 +498,10 @@ struct R8Bwd {
 // and the block writes its own line of partial sums, which r8_colsum_kernel adds
 // in a fixed order: the result does not depend on timing.
 // Blocks of 128 threads run four an SM: 153 registers a thread left three (65536 x
-// 1024 bf16: 102 us against 94).  Single loads keep their registers, and three.
+// 1024 bf16: 102 us against 94).  With single loads three run, and are launched:
+// without the bound their registers left two (65536 x 501 bf16: 144 us against 95).
 template <class EN, class EX, bool VEC, int NC, int U, int NT, int LPR = 32>
-__global__ void __launch_bounds__(NT, VEC && NT == 128 ? 4 : 1) r8_bwd_kernel(const R8Bwd p) {
+__global__ void __launch_bounds__(NT, NT != 128 ? 1 : VEC ? 4 : 3) r8_bwd_kernel(const R8Bwd p) {
     extern __shared__ float r8_acc[];  // blockDim.y x cols, when blockDim.y > 1
     __shared__ float2 part[R8_MAX_WARPS];
     constexpr int RPW = 32 / LPR;
