@@ -763,11 +763,12 @@ static int r8_fwd_check(const R8Fwd& p, int xt, int rt) {
     return MMB_OK;
 }
 
-// The backward's shape: fp32 gradients of three or four chunks take two warps a row
-// (65536 x 1024 fp32: 175 -> 157 us).
-static R8Shape r8_bwd_shape(int64_t cols, bool vec, bool f32) {
+// The backward's shape: with an fp32 stream (whatever the gradient of the norm is in),
+// three or four chunks take two warps a row (65536 x 1024 fp32: 175 -> 157 us; bf16
+// gradients, where one warp spilled: 153 -> 134).
+static R8Shape r8_bwd_shape(int64_t cols, bool vec, bool dx_f32) {
     const int64_t chunks = (cols + R8_CHUNK - 1) / R8_CHUNK;
-    return r8_shape(cols, vec && !(f32 && (chunks == 3 || chunks == 4)));
+    return r8_shape(cols, vec && !(dx_f32 && (chunks == 3 || chunks == 4)));
 }
 // Blocks of the backward: enough to fill the GPU, few enough that the lines of
 // partial sums stay small.
@@ -792,7 +793,7 @@ static int r8_bwd_launch(const R8Bwd& p, const R8Shape& s, int blocks, cudaStrea
         r8_bwd_kernel<EN, EX, VEC, 2, 2, 128><<<blocks, block, sm, st>>>(p);
     else if (s.nc == 2) r8_bwd_kernel<EN, EX, VEC, 2, VEC ? 2 : 1, 512><<<blocks, block, sm, st>>>(p);
     else if (s.warps > 1) r8_bwd_kernel<EN, EX, VEC, 4, 1, 512><<<blocks, block, sm, st>>>(p);
-    else if constexpr (VEC && sizeof(typename EN::T) == 2)
+    else if constexpr (VEC && sizeof(typename EX::T) == 2)
         r8_bwd_kernel<EN, EX, VEC, 4, 1, 128><<<blocks, block, sm, st>>>(p);
     return mmb_launch_status();
 }
@@ -867,7 +868,7 @@ extern "C" int mmb_norm_ck8_bwd(int64_t rows, int64_t cols, int32_t dn_type, con
     const int nb = r8_bytes(dn_type), xb = r8_bytes(dx_type);
     const bool vec = cols % 8 == 0 && r8_aligned(dn, lddn, nb) && r8_aligned(dh, lddh, xb) &&
                      r8_aligned(dx, lddx, xb) && r8_aligned(weight, 0, 4) && r8_aligned_q(q, ldq);
-    const R8Shape s = r8_bwd_shape(cols, vec, dn_type == MMB_F32);
+    const R8Shape s = r8_bwd_shape(cols, vec, dx_type == MMB_F32);
     if (!s.nc) return MMB_ERR_UNSUPPORTED;
     const int blocks = r8_bwd_blocks(rows, s, vec);
     int rc;

@@ -2,7 +2,8 @@
 
 The norm's backward launches as many blocks as are resident at once: four of 128 threads
 an SM with vector loads, three with single ones.  A kernel whose registers leave room for
-fewer makes the last of them wait for the others to end."""
+fewer makes the last of them wait for the others to end, and one that spills moves the
+spilled values through the memory that bounds it."""
 import os
 import re
 import subprocess
@@ -38,3 +39,10 @@ def test_blocks_of_the_backward_fit_side_by_side(backward_forms):
     for (a, b, vec, nc, threads), (regs, spill) in backward_forms.items():
         if threads == 128:
             assert regs * threads * (4 if vec else 3) <= REGISTERS, (a, b, vec, nc, regs)
+
+
+def test_rows_of_up_to_8192_columns_spill_nothing(backward_forms):
+    """Wider rows take four chunks in blocks of up to 512 threads, where some forms do."""
+    for form, (regs, spill) in backward_forms.items():
+        if form[3:] != (4, 512):
+            assert spill == 0, (form, spill)
