@@ -763,7 +763,9 @@ static bool w8_two_groups(int64_t M, int64_t N, int64_t K) {
 // with their number.
 template <class D>
 static int w8_seg(int out_type) {
-    return (D::F32 ? W8_SEG_FP32_DY : out_type == MMB_F32 ? W8_SEG_FP32_DW : W8_SEG_16_DW) / D::BT;
+    const int tokens = D::F32 ? W8_SEG_FP32_DY : out_type == MMB_F32 ? W8_SEG_FP32_DW
+                                               : W8_SEG_16_DW / D::PARTS;
+    return tokens / D::BT;
 }
 // Several slices, or sums that leave TMEM more than once and have no fp32 result to
 // gather in, go through the workspace.

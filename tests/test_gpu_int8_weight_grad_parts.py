@@ -165,3 +165,19 @@ def test_sums_gathered_in_the_result_or_the_workspace(M, out, normed):
         bound = 2.0 ** -17 * size + 2.0 ** -8 * want.abs() * (out != torch.float32) + 2e-4 * M ** 0.5
         assert float(bound.max()) < 10
         assert torch.all((dw[n, k].double() - want).abs() <= bound)
+
+
+def test_an_fp16_result_over_many_tokens_is_rounded_once():
+    """So many tiles that all tokens are one slice: what the accumulators truncate before
+    the sums leave them adds less than a hundredth to the result's own rounding."""
+    from momentummamba_b200 import int8
+    M, N, K = 65536, 8192, 8192
+    g = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(M, K, generator=g, device=DEV).half()
+    dy = torch.randn(M, N, generator=g, device=DEV).half()
+    ck = int8.checkpoint_rows(x)
+    del x
+    dw = int8.weight_grad_ckpt(dy, ck)
+    want, _ = products64(dy[:, :64], ck.restore(torch.bfloat16)[:, :2048], None, None)
+    ideal = float((want.half().double() - want).norm())
+    assert float((dw[:64, :2048].double() - want).norm()) <= 1.01 * ideal
