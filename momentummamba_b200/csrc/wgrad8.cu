@@ -71,15 +71,16 @@ __device__ __forceinline__ uint32_t w8_chunk(int block, int t, int c) {
 // accumulators; CW, EW: converter (in CG groups, each at a block of its own) and
 // epilogue warps.
 //
-// Two groups share each load of dy (65536 x (4096, 1024) bf16: 815 -> 560 us).
+// Two groups share each load of dy (65536 x (4096, 1024) bf16: 616 -> 477 us, in two
+// parts 1241 -> 860).
 //
 // What bounds it is shared memory: a block of 64 tokens of a 256 x 256 tile moves
 // 48 KB in by TMA, 16 KB out and 32 KB back through the converters and 96 KB into
 // the tensor cores, 192 KB or 1536 cycles at 128 bytes a cycle, against 1024 cycles
-// of MMAs.  B200: 65536 x (4096, 1024) bf16 460-478 us, 1.15-1.2e15 operations/s,
+// of MMAs.  B200: 65536 x (4096, 1024) bf16 466 us, slices added, 1.2e15 operations/s,
 // 0.72 of the measured bf16 rate (400 us with the converters left out); 76800 x
-// (1024, 256) bf16 60 us.  fp32, three parts: 76800 x (1024, 256) 158 us, 32768 x
-// (512, 128) 29 us.
+// (1024, 256) bf16 61 us.  fp32, three parts: 76800 x (1024, 256) 165 us, 32768 x
+// (512, 128) 29 us.  The plans of the large sizes give 128 units to 148 SMs.
 template <int GROUPS>
 struct W8Half {
     static constexpr bool F32 = false;
@@ -96,9 +97,9 @@ struct W8Half {
 //   * 16-bit dy, whose tiles are too large for registers: added where the result
 //     goes, in fp32.  Against 64 bits, random values: an fp32 result of bf16 dy is off
 //     by 1e-6 with 4096 tokens, 2.5e-6 with 8192 and 1.6e-5 with 32768, with dy in two
-//     parts by 6e-6, 1.1e-5 and 3.5e-5; 65536 x (4096, 1024) takes 565 us, 505 and 475
-//     (905, 870 and 860).  A 16-bit result is off by its own 1.65e-3 or 2.05e-4 in any
-//     case, and gathers 32768 tokens.
+//     parts by 6e-6 with 4096 and 1.1e-5 with 8192; 65536 x (4096, 1024) takes 560 us,
+//     505 and 470 (900 and 860).  A 16-bit result is off by its own 1.65e-3 or 2.05e-4
+//     in any case and gathers 32768 tokens, in two parts (fp16 results) half of that.
 constexpr int W8_SEG_FP32_DY = 1024, W8_SEG_FP32_DW = 4096, W8_SEG_16_DW = 32768;
 struct W8F32 {
     static constexpr bool F32 = true;
@@ -108,8 +109,9 @@ struct W8F32 {
 };
 // 16-bit dy (bf16 or fp16 in memory: BF) in two bf16 parts.  Blocks of 32 tokens
 // leave room for both parts of 256 columns.  Twice the MMAs of W8Half, and dy goes
-// through the converters: 65536 x (4096, 1024) bf16 880 us (one part 475), 76800 x
-// (1024, 256) 85 us (65).
+// through the converters: 65536 x (4096, 1024) bf16 852 us (one part 466), 76800 x
+// (1024, 256) 84 us (61).  A block of 32 tokens and two groups moves what W8Half's of 64
+// does, 192 KB against 1024 cycles of MMAs, and takes as long, 0.86 us.
 template <bool BF, int GROUPS>
 struct W8Two {
     static constexpr bool F32 = false;
@@ -728,7 +730,12 @@ __global__ void __launch_bounds__(W8_SUM_NT)
 // ---------------------------------------------------------------------------
 // Slices of the tokens: the count with the least estimated time, a round of
 // units costing its token blocks plus a tile's way out, and every slice one
-// more write and read of the result.
+// more write and read of the result.  The costs of blocks and tiles are weights, not
+// times: measured with 148 tiles of one slice, a block takes 0.51 us (fp32), 0.54 and
+// 0.86 (one part, one and two groups), 0.64 and 0.86 (two parts), a tile's start and way
+// out 8, 12 and 20.  With those figures 13 sizes took as long, up to 15 % longer
+// (8192 x (2048, 2048) bf16 85 -> 98 us) or 2 % less: rounds overlap, and slices share
+// dy in L2, which no cost here knows of.
 struct W8Plan {
     int64_t slices, blocks;
     double us;
