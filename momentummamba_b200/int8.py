@@ -285,7 +285,8 @@ def linear_q8(x: Q8Rows, w: Q8Rows, bias: Optional[torch.Tensor] = None,
               out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
     """x @ w^T (+ bias) of 8-bit rows: x (..., K), w (N, K) -> (..., N) in out_dtype.
 
-    Sums are exact integers (K <= 131071), scaled in fp32 and rounded once.
+    Sums are exact integers (K <= 131071), scaled in fp32 (by the token's scale, then
+    the channel's) and rounded once.
     Rows that do not start on 16-byte boundaries (quantize_rows and rms_norm_q8
     make ones that do) are copied first.  No gradient."""
     xq, wq, xs, ws = x.q, w.q, x.scale, w.scale
