@@ -534,8 +534,9 @@ int mmb_restore_q8(int64_t rows, int64_t cols, const int8_t* q, int64_t ldq, con
  *   out[m, n] = (sum_k x[m, k] w[n, k]) * xs[m] * ws[n] (+ bias[n])
  * x (M, K) tokens with a scale each, w (N, K) a weight with a scale per output
  * channel; exact integer sums (K <= 131071), fp32 scaling in the order written
- * (a sum * xs beyond fp32's range is an infinity), one rounding to out_type.  x and w 16-byte aligned, ldx and ldw multiples of 16; out has any
- * alignment.  bias nullable. */
+ * (a sum * xs beyond fp32's range is an infinity), one rounding to out_type.  x
+ * and w 16-byte aligned, ldx and ldw multiples of 16; out has any alignment.  bias
+ * nullable. */
 int mmb_gemm_q8(int64_t M, int64_t N, int64_t K, const int8_t* x, int64_t ldx, const float* xs,
                 const int8_t* w, int64_t ldw, const float* ws, const float* bias, int32_t out_type,
                 void* out, int64_t ldo, mmb_stream_t stream);
